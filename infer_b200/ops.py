@@ -9,8 +9,9 @@ from __future__ import annotations
 import collections
 import ctypes
 import functools
+import math
 import os
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -298,6 +299,158 @@ def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, seed: torch
     f = _fn("plain", "ib_sample_filtered", [c_void_p, c_int64, c_int64] + [c_void_p] * 9)
     _call(f, logits.data_ptr(), B, V, temperature.data_ptr(), seed.data_ptr(), step.data_ptr(), top_k.data_ptr(),
           top_p.data_ptr(), out.data_ptr(), _ptr(feedback), _ptr(slots), _stream())
+    return out
+
+
+# ----------------------------------------------------------------------------- log probabilities
+
+class TokenLogprobs(NamedTuple):
+    """What ``token_logprobs`` and ``head_logprobs`` return, one row a place: float32 [T], float32 [T], int32 [T, top], float32 [T, top]."""
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+@functools.lru_cache(maxsize=None)
+def max_top_logprobs() -> int:
+    """The most alternatives that a call may ask for."""
+    return int(_fn("score", "ib_max_top_logprobs", [])())
+
+
+def _check_logprobs(rows: int, device, tokens: Optional[torch.Tensor], top: int, scale: float, softcap: float, status: Optional[torch.Tensor]) -> int:
+    top = int(top)
+    if not 0 <= top <= max_top_logprobs():
+        raise KernelError(f"0 to {max_top_logprobs()} alternatives can be asked for, not {top}")
+    if not (scale > 0 and math.isfinite(scale)):
+        raise KernelError(f"the logits' scale must be positive and finite, not {scale}")
+    if not (softcap >= 0 and math.isfinite(softcap)):
+        raise KernelError(f"the logits' cap must be positive and finite, or 0 for none, not {softcap}")
+    for name, t, shape in (("tokens", tokens, (rows,)), ("status", status, (1,))):
+        if t is not None:
+            _check(t, name, torch.int32, shape)
+            if t.device != device:
+                raise KernelError(f"{name} must lie on {device}, not on {t.device}")
+    return top
+
+
+def _new_logprobs(rows: int, top: int, device) -> TokenLogprobs:
+    both = torch.empty((2, rows), dtype=torch.float32, device=device)
+    return TokenLogprobs(both[0], both[1], torch.empty((rows, top), dtype=torch.int32, device=device),
+                         torch.empty((rows, top), dtype=torch.float32, device=device))
+
+
+def _logprobs_cluster(rows: int, vocab: int, sm_count: int) -> int:
+    """CTAs that share a row of logits: while the rows alone leave the GPU idle, and each keeps a chunk of 8,192 elements."""
+    cluster = 8
+    while cluster > 1 and (rows * cluster > 4 * sm_count or vocab < 8192 * cluster // 2):
+        cluster //= 2
+    return cluster
+
+
+def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0, status: Optional[torch.Tensor] = None,
+                   scale: float = 1.0, softcap: float = 0.0, out: Optional[TokenLogprobs] = None) -> TokenLogprobs:
+    """How likely tokens are, from float32 logits [T, V], one row a place (as ``sample`` takes them): the log probability of ``tokens``
+    (int32 [T]; -1 or no ``tokens`` at all: none is asked for, the result is 0), the entropy of the row's distribution, and the ``top``
+    likeliest tokens (0 to 20) with their log probabilities, by falling logit, among equal logits the lowest id first. A logit of -inf has no
+    probability and is no alternative; places without an alternative hold id -1 and -inf. A row of -inf only: log probability -inf,
+    entropy 0. A NaN or +inf in a row makes its floats NaN (the ids follow the logits that are no NaN). Any other token outside
+    [0, V): NaN, and the status word (if given) is set to 1. ``scale`` / ``softcap``: the distribution is that of
+    softcap * tanh(logits * scale / softcap) (-inf stays -inf), or logits * scale without a cap; alternatives go by ``logits``.
+    Each call may run on any stream; a captured one reads its inputs anew at each replay."""
+    _check(logits, "logits", torch.float32)
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise KernelError(f"logits must be [rows, vocabulary], got {tuple(logits.shape)}")
+    T, V = logits.shape
+    top = _check_logprobs(T, logits.device, tokens, top, scale, softcap, status)
+    r = _new_logprobs(T, top, logits.device) if out is None else out
+    if T == 0:
+        return r
+    from . import fast_ops
+    f = _fn("score", "ib_token_logprobs", [c_void_p, c_int64, c_int64, c_void_p, c_int, c_float, c_float] + [c_void_p] * 4 + [c_int] + [c_void_p] * 2)
+    with torch.cuda.device(logits.device):
+        _call(f, logits.data_ptr(), T, V, _ptr(tokens), top, float(scale), float(softcap), r.logprob.data_ptr(), r.entropy.data_ptr(),
+              r.top_ids.data_ptr(), r.top_logprobs.data_ptr(), _logprobs_cluster(T, V, fast_ops.sm_count(logits.device)), _ptr(status), _stream())
+    return r
+
+
+def head_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0, scale: float = 1.0,
+                  softcap: float = 0.0, status: Optional[torch.Tensor] = None) -> TokenLogprobs:
+    """``token_logprobs`` of the logits x @ w.T (x [T, H], w [V, H], both bfloat16 or both float32; scaled and capped as there), which are
+    not kept: bfloat16 rows go through a kernel that holds them in tensor memory only; up to 16 rows, rows that do not keep to 16 bytes and
+    float32 go through logits of a few rows at a time. ``w`` is a loaded weight (as for ``linear``). A kernel whose bounded wait runs out
+    says so in the device's status word."""
+    _check(x, "x")
+    _check(w, "w", x.dtype)
+    dtype_code(x.dtype)
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or min(w.shape) < 1:
+        raise KernelError(f"head_logprobs: x is {tuple(x.shape)} but w is {tuple(w.shape)}")
+    if w.device != x.device:
+        raise KernelError(f"w must lie on {x.device}, not on {w.device}")
+    T, V = x.shape[0], w.shape[0]
+    top = _check_logprobs(T, x.device, tokens, top, scale, softcap, status)
+    from . import fast_ops
+    with torch.cuda.device(x.device):
+        if T > 0 and x.dtype == torch.bfloat16:
+            r = fast_ops.head_logprobs(x, w, tokens, top, scale, softcap, status)
+            if r is not None:
+                return r
+        r = _new_logprobs(T, top, x.device)
+        step = max(1, min(T, HEAD_LOGITS // V))
+        logits = torch.empty((step, V), dtype=torch.float32, device=x.device)
+        for lo in range(0, T, step):
+            hi = min(T, lo + step)
+            z = logits[:hi - lo]
+            if fast_ops.linear(x[lo:hi], w, None, None, torch.float32, z) is None:
+                linear_plain(x[lo:hi], w, out=z, w_ready=True)
+            token_logprobs(z, None if tokens is None else tokens[lo:hi], top, status, scale, softcap, TokenLogprobs(*(t[lo:hi] for t in r)))
+    return r
+
+
+# Elements of the logits that ``head_logprobs`` has in memory at a time where it needs them: 64 MB, which stay in L2.
+HEAD_LOGITS = 1 << 24
+
+ACTIVATIONS = {"none": 0, "relu": 1, "relu_squared": 2, "gelu_tanh": 3, "gelu": 4, "silu": 5}
+
+
+def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
+               residual: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out = residual + act(x @ w.T + bias), rounded once. x [M, K], w [N, K], both bfloat16 or both float32; bias float32 [N]; residual float32
+    [M, N] (may be ``out``); ``activation``: "none", "relu", "relu_squared" (max(z, 0)^2), "gelu_tanh"
+    (0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3)))), "gelu" (0.5 z (1 + erf(z / sqrt 2))), "silu" (z / (1 + e^-z)). The result is
+    float32 or bfloat16 (default: as x; with a residual float32). ``w`` is a loaded weight (as for ``linear``). A kernel whose bounded wait
+    runs out says so in the device's status word."""
+    _check(x, "x")
+    _check(w, "w", x.dtype)
+    dtype_code(x.dtype)
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or min(w.shape) < 1:
+        raise KernelError(f"linear_act: x is {tuple(x.shape)} but w is {tuple(w.shape)}")
+    if activation not in ACTIVATIONS:
+        raise KernelError(f"activation {activation!r} is not among {sorted(ACTIVATIONS)}")
+    (M, K), N = x.shape, w.shape[0]
+    if bias is not None:
+        _check(bias, "bias", torch.float32, (N,))
+    if residual is not None:
+        _check(residual, "residual", torch.float32, (M, N))
+    if out_dtype is None:
+        out_dtype = out.dtype if out is not None else torch.float32 if residual is not None else x.dtype
+    dtype_code(out_dtype)
+    if out is not None:
+        _check(out, "out", out_dtype, (M, N))
+    for name, t in (("w", w), ("bias", bias), ("residual", residual), ("out", out)):
+        if t is not None and t.device != x.device:
+            raise KernelError(f"{name} must lie on {x.device}, not on {t.device}")
+    with torch.cuda.device(x.device):
+        if out is None:
+            out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+        if out.numel() == 0:
+            return out
+        from . import fast_ops
+        z = fast_ops.linear(x, w, bias, None, torch.float32, None)
+        if z is None:
+            z = linear_plain(x, w, bias, None, torch.float32, w_ready=True)
+        f = _fn("score", "ib_act_residual", [c_void_p] * 3 + [c_int64, c_int, c_int, c_void_p])
+        _call(f, z.data_ptr(), _ptr(residual), out.data_ptr(), M * N, ACTIVATIONS[activation], dtype_code(out_dtype), _stream())
     return out
 
 
