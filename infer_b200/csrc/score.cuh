@@ -20,27 +20,55 @@ __device__ __forceinline__ float logit(float z, float scale, float cap) {
     return cap > 0.0f && l != -INFINITY ? cap * tanhf(l / cap) : l;
 }
 
-// m = max l, s = sum exp(l - m), d = sum exp(l - m) (l - m) of the elements seen. Only the differences l - m are ever scaled or exponentiated,
-// so that logprob keeps its digits where one token has nearly all of the probability.
+// The logits of N sums under a cap, without tanhf's branches: for |u| <= 0.6 an odd polynomial (a minimax fit of tanh(u) / u in u^2, off by
+// 2.5e-9 before its roundings: 2 x 2^-24 of the result with them), else 1 - 2 / (1 + e^2|u|) (5 x 2^-24). A thread goes by the largest of its own.
+template <int N> __device__ __forceinline__ void cap_logits(float (&l)[N], const float (&z)[N], float scale, float cap) {
+    const float to_u = scale / cap;
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) { l[i] = z[i] * to_u; most = fmaxf(most, l[i] == -INFINITY ? 0.0f : fabsf(l[i])); }
+    if (most <= 0.6f) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float u = l[i], q = u * u;
+            float t = fmaf(q, -0.005852164700627327f, 0.02075362578034401f);
+            t = fmaf(q, t, -0.05376870185136795f);
+            t = fmaf(q, t, 0.13331688940525055f);
+            t = fmaf(q, t, -0.3333328366279602f);
+            t = fmaf(q, t, 1.0f);
+            l[i] = u == -INFINITY ? u : cap * (u * t);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float u = l[i], t = 1.0f - __fdividef(2.0f, 1.0f + exp2_fast(fabsf(u) * (2.0f * LOG2E)));
+            l[i] = u == -INFINITY ? u : cap * copysignf(t, u);
+        }
+    }
+}
+
+// m = max l, s = sum exp(l - m), d = sum exp(l - m) (l - m) of the elements seen. Only the differences l - m are ever exponentiated, so that
+// logprob keeps its digits where one token has nearly all of the probability.
 struct Stats {
     float m, s, d;
     __device__ __forceinline__ void clear() { m = -INFINITY; s = 0.0f; d = 0.0f; }
-    __device__ __forceinline__ void raise(float to) {        // to >= m, or m is NaN's neighbour: s says so already
+    __device__ __forceinline__ void raise(float to) {        // to > m
         const float x = m - to, f = s != 0.0f ? exp2_fast(x * LOG2E) : 0.0f;
         d = f > 0.0f ? f * fmaf(x, s, d) : (f == 0.0f ? 0.0f : f);
         s *= f;
         m = to;
     }
-    template <int N> __device__ __forceinline__ void add(const float (&l)[N]) {
-        float top = l[0];
+    template <int N> __device__ __forceinline__ void add(const float (&z)[N], float scale = 1.0f) {
+        float top = z[0];
 #pragma unroll
-        for (int i = 1; i < N; i++) top = fmaxf(top, l[i]);
+        for (int i = 1; i < N; i++) top = fmaxf(top, z[i]);
+        top *= scale;
         if (top > m) raise(top);
         const float ref = m == -INFINITY ? 0.0f : m;
         float s0 = 0.0f, s1 = 0.0f, d0 = 0.0f, d1 = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const float x = l[i] - ref, e = exp2_fast(x * LOG2E);
+            const float x = fmaf(z[i], scale, -ref), e = exp2_fast(x * LOG2E);
             // (an element of -inf: e = 0, and 0 * -1000 adds nothing; a NaN goes into s, which is enough)
             if (i & 1) { s1 += e; d1 = fmaf(e, fmaxf(x, -1000.0f), d1); } else { s0 += e; d0 = fmaf(e, fmaxf(x, -1000.0f), d0); }
         }
@@ -52,8 +80,9 @@ struct Stats {
         s += o.s;
         d += o.d;
     }
-    __device__ __forceinline__ float logprob(float l) const {
-        return m == -INFINITY && s == 0.0f ? -INFINITY : (l - m) - logf(s);
+    // of the logit z scale: its distance from m is formed as add() formed the others'
+    __device__ __forceinline__ float logprob(float z, float scale = 1.0f) const {
+        return m == -INFINITY && s == 0.0f ? -INFINITY : fmaf(z, scale, -m) - logf(s);
     }
     __device__ __forceinline__ float entropy() const { return m == -INFINITY && s == 0.0f ? 0.0f : logf(s) - d / s; }
 };
@@ -70,12 +99,16 @@ __device__ __forceinline__ Stats warp_join(Stats v) {
     return v;
 }
 
-__device__ __forceinline__ void finish(const Stats& st, int token, float at, int64_t vocab, float* logprob, float* entropy, int* status) {
+// (at: the token's sum z)
+__device__ __forceinline__ float logprob_of(const Stats& st, float z, float scale, float cap) {
+    return cap > 0.0f ? st.logprob(logit(z, scale, cap)) : st.logprob(z, scale);
+}
+__device__ __forceinline__ void finish(const Stats& st, int token, float at, float scale, float cap, int64_t vocab, float* logprob, float* entropy, int* status) {
     if (entropy) *entropy = st.entropy();
     if (!logprob) return;
     const bool none = token == -1, outside = !none && (token < 0 || token >= vocab);
     if (outside && status) atomicExch(status, 1);
-    *logprob = none ? 0.0f : outside ? __int_as_float(0x7fc00000) : st.logprob(at);
+    *logprob = none ? 0.0f : outside ? __int_as_float(0x7fc00000) : logprob_of(st, at, scale, cap);
 }
 
 // A key orders alternatives: a larger logit first, among equal ones a lower id (-0 is 0). Every key of an element is above 0.

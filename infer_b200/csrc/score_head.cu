@@ -108,22 +108,39 @@ template <int N> struct Best {
         for (int i = 0; i < N; i++) { v[i] = -INFINITY; id[i] = -1; }
     }
     __device__ __forceinline__ bool wants(float z) const { return z > v[N - 1]; }
-    __device__ __forceinline__ void put(float z, int n) {            // wants(z); ids come in ascending order
-        bool above = true;                                            // z > v[i]
+    __device__ __forceinline__ void put(bool mine, float z, int n) { // mine: wants(z); among equal values ids come in ascending order
+        bool above = mine;                                            // z > v[i]
 #pragma unroll
         for (int i = N - 1; i > 0; i--) {
-            const bool next = z > v[i - 1];
+            const bool next = mine && z > v[i - 1];
             v[i] = next ? v[i - 1] : (above ? z : v[i]);
             id[i] = next ? id[i - 1] : (above ? n : id[i]);
             above = next;
         }
-        if (above) { v[0] = z; id[0] = n; }
+        v[0] = above ? z : v[0];
+        id[0] = above ? n : id[0];
+    }
+    // Takes what it wants of 32 neighbouring columns, the largest first (z is used up). One branch for the warp and a round for as many columns as
+    // a lane wants: with a branch for each column and lane a single warp on its scheduler waited for most of its time.
+    __device__ __forceinline__ void take(float (&z)[32], int n0) {
+        for (;;) {
+            float top = z[0];
+#pragma unroll
+            for (int j = 1; j < 32; j++) top = fmaxf(top, z[j]);
+            const bool mine = wants(top);
+            if (!__any_sync(0xffffffffu, mine)) return;
+            int at = 0;
+#pragma unroll
+            for (int j = 31; j >= 0; j--) at = z[j] == top ? j : at;
+            put(mine, top, n0 + at);
+#pragma unroll
+            for (int j = 0; j < 32; j++) z[j] = at == j ? -INFINITY : z[j];
+        }
     }
 };
 template <> struct Best<0> {
     __device__ __forceinline__ void clear() {}
-    __device__ __forceinline__ bool wants(float) const { return false; }
-    __device__ __forceinline__ void put(float, int) {}
+    __device__ __forceinline__ void take(float (&)[32], int) {}
 };
 
 struct HeadParams {
@@ -299,30 +316,14 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                             for (int j = 0; j < 32; j++) found = token - n0 == j ? z[j] : found;
                             p.at[row] = found;
                         }
-                        if constexpr (N > 0) {
-                            float top = z[0];
-#pragma unroll
-                            for (int j = 1; j < 32; j++) top = fmaxf(top, z[j]);
-                            if (best.wants(top)) {
-#pragma unroll 1
-                                for (int j0 = 0; j0 < 32; j0 += 8) {
-                                    float part[8];
-#pragma unroll
-                                    for (int j = 0; j < 8; j++) part[j] = j0 == 0 ? z[j] : j0 == 8 ? z[8 + j] : j0 == 16 ? z[16 + j] : z[24 + j];
-#pragma unroll
-                                    for (int j = 0; j < 8; j++)
-                                        if (best.wants(part[j])) best.put(part[j], n0 + j0 + j);
-                                }
-                            }
-                        }
                         if (p.cap > 0.0f) {
-#pragma unroll
-                            for (int j = 0; j < 32; j++) z[j] = ib::score::logit(z[j], p.scale, p.cap);
-                        } else if (p.scale != 1.0f) {
-#pragma unroll
-                            for (int j = 0; j < 32; j++) z[j] *= p.scale;
+                            float l[32];
+                            ib::score::cap_logits<32>(l, z, p.scale, p.cap);
+                            st.add<32>(l);
+                        } else {
+                            st.add<32>(z, p.scale);
                         }
-                        st.add<32>(z);
+                        best.take(z, n0);
                     }
                 }
                 tc_fence_before();
@@ -398,7 +399,7 @@ join_chunks_kernel(const JoinParams p) {
             total = st;
             const int token = p.tokens ? p.tokens[row] : -1;
             const float at = token >= 0 && token < p.V ? p.at[row] : 0.0f;
-            ib::score::finish(st, token, ib::score::logit(at, p.scale, p.cap), p.V, p.logprob + row, p.entropy + row, p.status);
+            ib::score::finish(st, token, at, p.scale, p.cap, p.V, p.logprob + row, p.entropy + row, p.status);
         }
     }
     if (p.top == 0) return;
@@ -443,7 +444,7 @@ join_chunks_kernel(const JoinParams p) {
         for (int j = 0; j < n; j++) above += found[j] > k;
         if (above < p.top) {
             p.top_ids[row * p.top + above] = int(ib::score::key_id(k));
-            p.top_logprobs[row * p.top + above] = st.logprob(ib::score::logit(ib::score::key_value(k), p.scale, p.cap));
+            p.top_logprobs[row * p.top + above] = ib::score::logprob_of(st, ib::score::key_value(k), p.scale, p.cap);
         }
     }
     for (int i = n + threadIdx.x; i < p.top; i += JOIN_THREADS) {

@@ -19,17 +19,19 @@ using ib::score::Stats;
 using bf16 = __nv_bfloat16;
 
 // ------------------------------------------------------------------------------------------------ from logits
-// A row is shared by the CTAs of a cluster, each taking a contiguous slice in chunks of THREADS x 16 elements; a thread holds four
-// 16-byte units of a chunk, and the next chunk's are requested before this one is looked at.  The statistics need no barrier until
-// the end.  For the alternatives a CTA keeps the best `top` keys of what it has seen, sorted, in shared memory; a chunk in which no element
-// beats the last of them costs one barrier.  Otherwise what beats it is appended behind the list, every entry counts the entries that
-// beat it, and those beaten by fewer than `top` are the new list.  In a first chunk nearly everything would be appended, so there a
-// lower bound comes first: of the 32 half-warps' best keys the top-th; only `top` half-warps hold keys that reach it, so that
-// MAX_TOP x 256 places are enough whatever the row holds.
-constexpr int THREADS = 512, UNITS = 4;
-constexpr int MAX_TOP = ib::score::MAX_TOP, GROUPS = THREADS / 16;
-constexpr int ROOM = MAX_TOP + MAX_TOP * 16 * 4 * UNITS;                 // the list, and what one chunk may append
-static_assert(GROUPS == 32, "a warp compares the half-warps' best keys");
+// A row is shared by the CTAs of a cluster, each taking a contiguous slice. A thread takes every THREADS-th 16-byte unit, four at a time, and
+// the next four are requested before these are looked at; the statistics need no barrier until the end.
+// The alternatives cost the stream one comparison for four units (the thread's largest element and its id): the `top` best of all elements
+// lie with at most `top` threads, those whose largest reaches the top-th largest of the threads'.  A bound on that is enough: the top-th
+// of the largest of 64 groups of 8 threads.  The elements of the few threads that reach it are read again (from L2), those that
+// reach the bound themselves go into shared memory beside the list of what came before, and every entry counts the entries that beat it.
+// A slice goes in segments, so that the room in shared memory is enough whatever the row holds: where the bound lets through more
+// threads than fit, the threads' own keys are compared and exactly `top` remain.
+constexpr int THREADS = 512, UNITS = 4, GROUPS = THREADS / 8;
+constexpr int SEGMENT = 48;                                              // units of a thread in a segment
+constexpr int MAX_TOP = ib::score::MAX_TOP;
+constexpr int ROOM = 5120;                                               // keys of a segment's candidates
+static_assert(ROOM >= MAX_TOP * SEGMENT * 4 && SEGMENT % UNITS == 0 && MAX_TOP <= GROUPS, "the candidates fit");
 
 struct Params {
     const float* logits;
@@ -44,14 +46,28 @@ struct Params {
     int* status;                 // or null
 };
 
+// Entries i of keys[0, n) that fewer than `top` others beat, called with (how many beat it, the key) by one thread each. Unequal keys, 0: none.
+template <typename F> __device__ __forceinline__ void ranked(const unsigned long long* keys, int n, int top, F&& put) {
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+        const unsigned long long k = keys[i];
+        int above = 0, j = 0;
+        for (; j + 4 <= n; j += 4) {
+            const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(keys + j), b = *reinterpret_cast<const ulonglong2*>(keys + j + 2);
+            above += (a.x > k) + (a.y > k) + (b.x > k) + (b.y > k);
+        }
+        for (; j < n; j++) above += keys[j] > k;
+        if (k != 0 && above < top) put(above, k);
+    }
+}
+
 template <int CL, bool TOP>
 __global__ void __launch_bounds__(THREADS, 2)
 token_logprobs_kernel(const Params p) {
-    extern __shared__ __align__(16) unsigned long long keys[];           // TOP: [ROOM], then the new list [MAX_TOP]
+    extern __shared__ __align__(16) unsigned long long keys[];           // TOP: the list [MAX_TOP], candidates [ROOM], the new list [MAX_TOP]
     __shared__ Stats red[THREADS / 32];
     __shared__ Stats parts[CL];                                           // of the cluster's CTAs, in the first
-    __shared__ unsigned long long lists[TOP ? CL * MAX_TOP : 1];
-    __shared__ unsigned long long best[GROUPS];
+    __shared__ __align__(16) unsigned long long lists[TOP ? CL * MAX_TOP : 1];
+    __shared__ unsigned long long best[TOP ? GROUPS : 1], bound;
     __shared__ int n_keys;
     const int rank = CL > 1 ? int(cg::this_cluster().block_rank()) : 0;
     const int64_t b = blockIdx.x / CL;
@@ -60,109 +76,131 @@ token_logprobs_kernel(const Params p) {
     // the row's first element sits `ahead` floats behind a 16-byte boundary: units are counted from that boundary
     const int ahead = int((reinterpret_cast<uintptr_t>(row) >> 2) & 3);
     const int64_t n_units = (p.vocab + ahead + 3) / 4;
-    const int64_t per = ((n_units + CL - 1) / CL + 31) / 32 * 32, u_lo = min(n_units, per * rank), u_hi = min(n_units, u_lo + per);
-    const int n_chunks = int((u_hi - u_lo + THREADS * UNITS - 1) / (THREADS * UNITS));
+    const int64_t per = (n_units + CL - 1) / CL, u_lo = min(n_units, per * rank);
+    const int mine = int(min(n_units, u_lo + per) - u_lo);                // units of this CTA
+    unsigned long long* found = keys + MAX_TOP;
     if (TOP) {
-        if (threadIdx.x < MAX_TOP) keys[threadIdx.x] = keys[ROOM + threadIdx.x] = 0;
-        if (threadIdx.x == 0) n_keys = 0;
+        if (threadIdx.x < MAX_TOP) keys[threadIdx.x] = keys[MAX_TOP + ROOM + threadIdx.x] = 0;
+        if (threadIdx.x == 0) { n_keys = 0; bound = 0; }
         __syncthreads();
     }
     if (CL > 1) cg::this_cluster().barrier_arrive();                      // (waited for before another CTA's shared memory is written)
     ib::pdl_wait();
-    const bool asked = rank == 0 && threadIdx.x == 0;
     int token = -1;
     float at = 0.0f;
-    if (asked && p.tokens) {
+    if (rank == 0 && threadIdx.x == 0 && p.tokens) {
         token = p.tokens[b];
         if (token >= 0 && token < p.vocab) at = row[token];
     }
-    auto fetch = [&](int chunk, float (&v)[UNITS * 4]) {
-#pragma unroll
-        for (int j = 0; j < UNITS; j++) {
-            const int64_t u = u_lo + int64_t(chunk) * (THREADS * UNITS) + j * THREADS + threadIdx.x, e = 4 * u - ahead;
-            if (u < u_hi && e >= 0 && e + 4 <= p.vocab) {
-                const float4 f = __ldcs(reinterpret_cast<const float4*>(row + e));
-                v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; k++) v[4 * j + k] = u < u_hi && e + k >= 0 && e + k < p.vocab ? row[e + k] : -INFINITY;
-            }
+    // unit i of this CTA: four elements, those outside the row as -inf
+    auto fetch = [&](int i) {
+        const int64_t e = 4 * (u_lo + i) - ahead;
+        float4 f;
+        if (i < mine && e >= 0 && e + 4 <= p.vocab) f = *reinterpret_cast<const float4*>(row + e);
+        else {
+            const bool in = i < mine;
+            f.x = in && e >= 0 && e < p.vocab ? row[e] : -INFINITY;
+            f.y = in && e + 1 >= 0 && e + 1 < p.vocab ? row[e + 1] : -INFINITY;
+            f.z = in && e + 2 >= 0 && e + 2 < p.vocab ? row[e + 2] : -INFINITY;
+            f.w = in && e + 3 < p.vocab ? row[e + 3] : -INFINITY;
         }
+        return f;
     };
+    auto id_of = [&](int i, int k) { return uint32_t(4 * (u_lo + i) - ahead + k); };
     Stats st;
     st.clear();
-    float next[UNITS * 4];
-    if (n_chunks > 0) fetch(0, next);
-    for (int chunk = 0; chunk < n_chunks; chunk++) {
-        float z[UNITS * 4];
+    float4 next[UNITS];
 #pragma unroll
-        for (int i = 0; i < UNITS * 4; i++) z[i] = next[i];
-        if (chunk + 1 < n_chunks) fetch(chunk + 1, next);
-        if (TOP) {
-            // (keys are made where they are needed: 64-bit comparisons of 16 elements would cost more than the statistics)
-            const int64_t e0 = 4 * (u_lo + int64_t(chunk) * (THREADS * UNITS) + threadIdx.x) - ahead;
-            auto key_of = [&](int i) { return ib::score::key(z[i], uint32_t(e0 + int64_t(i / 4) * (THREADS * 4) + (i & 3))); };
-            const unsigned long long last = keys[p.top - 1];              // 0: fewer than top so far
-            const float floor = last ? ib::score::key_value(last) : -INFINITY;
-            bool any = false;
+    for (int j = 0; j < UNITS; j++) next[j] = fetch(j * THREADS + int(threadIdx.x));
+    for (int s0 = 0; s0 < mine; s0 += SEGMENT * THREADS) {
+        const int s1 = min(mine, s0 + SEGMENT * THREADS);
+        float largest = -INFINITY;
+        int largest_at = 0;                                               // unit (in the CTA) x 4 + element
+        for (int i0 = s0; i0 < s1; i0 += UNITS * THREADS) {
+            float z[UNITS * 4];
 #pragma unroll
-            for (int i = 0; i < UNITS * 4; i++) any |= z[i] > floor;         // (an equal one has a higher id than what is in the list)
-            const int busy = __syncthreads_count(any);
-            if (busy) {
-                unsigned long long bound = last + 1;
-                if (busy * (UNITS * 4) > ROOM - MAX_TOP) {
-                    unsigned long long mine = 0;
+            for (int j = 0; j < UNITS; j++) { z[4 * j] = next[j].x; z[4 * j + 1] = next[j].y; z[4 * j + 2] = next[j].z; z[4 * j + 3] = next[j].w; }
 #pragma unroll
-                    for (int i = 0; i < UNITS * 4; i++)
-                        if (z[i] > -INFINITY) { const unsigned long long k = key_of(i); mine = k > mine ? k : mine; }
+            for (int j = 0; j < UNITS; j++) next[j] = fetch(i0 + (UNITS + j) * THREADS + int(threadIdx.x));
+            if (TOP) {
+                float m = z[0];
 #pragma unroll
-                    for (int o = 8; o > 0; o >>= 1) {
-                        const unsigned long long other = __shfl_xor_sync(0xffffffffu, mine, o);
-                        mine = other > mine ? other : mine;
-                    }
-                    if ((lane & 15) == 0) best[threadIdx.x >> 4] = mine;
-                    __syncthreads();
-                    const unsigned long long g = best[lane];
-                    int beaten = 0;
+                for (int i = 1; i < UNITS * 4; i++) m = fmaxf(m, z[i]);
+                if (m > largest) {
+                    largest = m;
+                    int which = 0;
 #pragma unroll
-                    for (int o = 0; o < 32; o++) { const unsigned long long other = __shfl_sync(0xffffffffu, g, o); beaten += other > g || (other == g && o < lane); }
-                    const unsigned int who = __ballot_sync(0xffffffffu, beaten == p.top - 1);
-                    const unsigned long long kth = __shfl_sync(0xffffffffu, g, __ffs(who) - 1);
-                    bound = kth > bound ? kth : bound;
+                    for (int i = UNITS * 4 - 1; i >= 0; i--) which = z[i] == m ? i : which;
+                    largest_at = 4 * (i0 + (which >> 2) * THREADS + int(threadIdx.x)) + (which & 3);
                 }
-                if (any) {
-#pragma unroll
-                    for (int i = 0; i < UNITS * 4; i++) {
-                        if (!(z[i] > -INFINITY)) continue;
-                        const unsigned long long k = key_of(i);
-                        if (k >= bound) keys[MAX_TOP + atomicAdd(&n_keys, 1)] = k;
-                    }
-                }
-                __syncthreads();
-                const int n = MAX_TOP + n_keys;
-                for (int i = threadIdx.x; i < n; i += THREADS) {
-                    const unsigned long long k = keys[i];
-                    if (k == 0) continue;
-                    int above = 0;
-                    for (int j = 0; j < n; j++) above += keys[j] > k;
-                    if (above < p.top) keys[ROOM + above] = k;
-                }
-                __syncthreads();
-                if (threadIdx.x < p.top) keys[threadIdx.x] = keys[ROOM + threadIdx.x];
-                if (threadIdx.x == 0) n_keys = 0;
-                __syncthreads();
-                if (threadIdx.x < MAX_TOP) keys[ROOM + threadIdx.x] = 0;
-                // (read again only behind the next chunk's barrier)
+            }
+            if (p.cap > 0.0f) {
+                float l[UNITS * 4];
+                ib::score::cap_logits<UNITS * 4>(l, z, p.scale, p.cap);
+                st.add<UNITS * 4>(l);
+            } else {
+                st.add<UNITS * 4>(z, p.scale);
             }
         }
-        if (p.cap > 0.0f) {
+        if (TOP) {
+            const unsigned long long last = keys[p.top - 1];              // 0: fewer than top so far
+            const unsigned long long mine_best = largest > -INFINITY ? ib::score::key(largest, id_of(largest_at >> 2, largest_at & 3)) : 0;
+            bool in = mine_best > last;
+            if (__syncthreads_count(in) == 0) continue;
+            unsigned long long g = mine_best;
 #pragma unroll
-            for (int i = 0; i < UNITS * 4; i++) z[i] = ib::score::logit(z[i], p.scale, p.cap);
-        } else if (p.scale != 1.0f) {
+            for (int o = 4; o > 0; o >>= 1) {
+                const unsigned long long other = __shfl_xor_sync(0xffffffffu, g, o);
+                g = other > g ? other : g;
+            }
+            if ((lane & 7) == 0) best[threadIdx.x >> 3] = g;
+            __syncthreads();
+            const unsigned long long g0 = best[lane], g1 = best[lane + 32];
 #pragma unroll
-            for (int i = 0; i < UNITS * 4; i++) z[i] *= p.scale;
+            for (int i = 0; i < GROUPS / (THREADS / 32); i++) {           // a warp looks where a few of the groups stand among all
+                const unsigned long long k = best[warp * (GROUPS / (THREADS / 32)) + i];
+                const int above = __popc(__ballot_sync(0xffffffffu, g0 > k)) + __popc(__ballot_sync(0xffffffffu, g1 > k));
+                if (lane == 0 && k != 0 && above == p.top - 1) bound = k;
+            }
+            __syncthreads();
+            unsigned long long least = max(bound, last + 1);
+            in = mine_best >= least;
+            const int reach = (s1 - s0 + THREADS - 1) / THREADS;          // units of a thread
+            if (__syncthreads_count(in) * reach * 4 > ROOM) {
+                if (in) found[atomicAdd(&n_keys, 1)] = mine_best;
+                __syncthreads();
+                ranked(found, n_keys, p.top, [&](int above, unsigned long long k) { if (above == p.top - 1) bound = k; });
+                __syncthreads();
+                least = max(bound, last + 1);
+                in = mine_best >= least;
+                if (threadIdx.x == 0) n_keys = 0;
+                __syncthreads();
+            }
+            // a warp reads its chosen threads' units again, a thread at a time
+            for (uint32_t todo = __ballot_sync(0xffffffffu, in); todo; todo &= todo - 1) {
+                const int t = warp * 32 + __ffs(todo) - 1;
+                for (int j = lane; j < reach; j += 32) {
+                    const int i = s0 + j * THREADS + t;
+                    if (i >= s1) break;
+                    const float4 f = fetch(i);
+                    const float v[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const unsigned long long key = v[k] > -INFINITY ? ib::score::key(v[k], id_of(i, k)) : 0;
+                        if (key >= least) found[atomicAdd(&n_keys, 1)] = key;
+                    }
+                }
+            }
+            __syncthreads();
+            ranked(keys, MAX_TOP + n_keys, p.top, [&](int above, unsigned long long k) { keys[MAX_TOP + ROOM + above] = k; });
+            __syncthreads();
+            if (threadIdx.x < MAX_TOP) {
+                keys[threadIdx.x] = keys[MAX_TOP + ROOM + threadIdx.x];
+                keys[MAX_TOP + ROOM + threadIdx.x] = 0;
+            }
+            if (threadIdx.x == 0) { n_keys = 0; bound = 0; }
+            __syncthreads();
         }
-        st.add<UNITS * 4>(z);
     }
     ib::pdl_launch_dependents();
     st = ib::score::warp_join(st);
@@ -177,7 +215,7 @@ token_logprobs_kernel(const Params p) {
         auto cluster = cg::this_cluster();
         cluster.barrier_wait();
         if (threadIdx.x == 0) *cluster.map_shared_rank(&parts[rank], 0) = st;
-        if (TOP) for (int i = threadIdx.x; i < MAX_TOP; i += THREADS) *cluster.map_shared_rank(&lists[rank * MAX_TOP + i], 0) = i < p.top ? keys[i] : 0;
+        if (TOP && threadIdx.x < p.top) *cluster.map_shared_rank(&lists[rank * p.top + threadIdx.x], 0) = keys[threadIdx.x];
         cluster.sync();
         if (rank != 0) return;
         if (warp == 0) {
@@ -188,25 +226,18 @@ token_logprobs_kernel(const Params p) {
     }
     if (threadIdx.x == 0) {
         red[0] = st;
-        ib::score::finish(st, token, ib::score::logit(at, p.scale, p.cap), p.vocab, p.logprob ? p.logprob + b : nullptr, p.entropy ? p.entropy + b : nullptr, p.status);
+        ib::score::finish(st, token, at, p.scale, p.cap, p.vocab, p.logprob + b, p.entropy + b, p.status);
     }
     if (TOP) {
         __syncthreads();
         st = red[0];
-        const unsigned long long* all = CL > 1 ? lists : keys;
-        const int n = CL > 1 ? CL * MAX_TOP : MAX_TOP;
-        int found = 0;
-        if (threadIdx.x < n) {
-            const unsigned long long k = all[threadIdx.x];
-            int above = 0;
-            for (int j = 0; j < n; j++) above += all[j] > k;
-            found = k != 0 && above < p.top;
-            if (found) {
-                p.top_ids[b * p.top + above] = int(ib::score::key_id(k));
-                p.top_logprobs[b * p.top + above] = st.logprob(ib::score::logit(ib::score::key_value(k), p.scale, p.cap));
-            }
-        }
-        const int filled = __syncthreads_count(found);
+        bool any = false;
+        ranked(CL > 1 ? lists : keys, CL > 1 ? CL * p.top : MAX_TOP, p.top, [&](int above, unsigned long long k) {
+            any = true;
+            p.top_ids[b * p.top + above] = int(ib::score::key_id(k));
+            p.top_logprobs[b * p.top + above] = ib::score::logprob_of(st, ib::score::key_value(k), p.scale, p.cap);
+        });
+        const int filled = __syncthreads_count(any);                      // (CL x MAX_TOP entries: a thread has one at most)
         if (threadIdx.x >= filled && threadIdx.x < p.top) {
             p.top_ids[b * p.top + threadIdx.x] = -1;
             p.top_logprobs[b * p.top + threadIdx.x] = -INFINITY;
@@ -216,7 +247,7 @@ token_logprobs_kernel(const Params p) {
 
 template <int CL, bool TOP>
 int launch_logprobs(const Params& p, int64_t rows, cudaStream_t stream) {
-    const size_t smem = TOP ? size_t(ROOM + MAX_TOP) * 8 : 0;
+    const size_t smem = TOP ? size_t(ROOM + 2 * MAX_TOP) * 8 : 0;
     static ib::PerDevice allowed;
     if (const int rc = ib::allow_smem(allowed, "token_logprobs", token_logprobs_kernel<CL, TOP>, smem)) return rc;
     return ib::launch("token_logprobs", token_logprobs_kernel<CL, TOP>, dim3(unsigned(rows * CL)), dim3(THREADS), smem, stream, CL, p);
