@@ -122,11 +122,8 @@ template <int N> struct Best {
     }
     // Takes what it wants of 32 neighbouring columns, the largest first (z is used up). One branch for the warp and a round for as many columns as
     // a lane wants: with a branch for each column and lane a single warp on its scheduler waited for most of its time.
-    __device__ __forceinline__ void take(float (&z)[32], int n0) {
-        for (;;) {
-            float top = z[0];
-#pragma unroll
-            for (int j = 1; j < 32; j++) top = fmaxf(top, z[j]);
+    __device__ __forceinline__ void take(float (&z)[32], float top, int n0) {
+        for (;; top = ib::score::largest_of<32>(z)) {
             const bool mine = wants(top);
             if (!__any_sync(0xffffffffu, mine)) return;
             int at = 0;
@@ -140,7 +137,7 @@ template <int N> struct Best {
 };
 template <> struct Best<0> {
     __device__ __forceinline__ void clear() {}
-    __device__ __forceinline__ void take(float (&)[32], int) {}
+    __device__ __forceinline__ void take(float (&)[32], float, int) {}
 };
 
 struct HeadParams {
@@ -319,11 +316,13 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                         if (p.cap > 0.0f) {
                             float l[32];
                             ib::score::cap_logits<32>(l, z, p.scale, p.cap);
-                            st.add<32>(l);
+                            st.add<32>(l, ib::score::largest_of<32>(l));
+                            best.take(z, ib::score::largest_of<32>(z), n0);
                         } else {
-                            st.add<32>(z, p.scale);
+                            const float top = ib::score::largest_of<32>(z);
+                            st.add<32>(z, top, p.scale);
+                            best.take(z, top, n0);
                         }
-                        best.take(z, n0);
                     }
                 }
                 tc_fence_before();
@@ -386,15 +385,19 @@ join_chunks_kernel(const JoinParams p) {
     ib::pdl_wait();
     ib::pdl_launch_dependents();
     if (warp == 0) {
-        Stats st;
-        st.clear();
+        float m = -INFINITY;
+        for (int c = lane; c < p.chunks; c += 32) m = fmaxf(m, p.stats[int64_t(c) * p.T + row].x);
+        m = ib::warp_max(m);
+        Stats st{m, 0.0f, 0.0f};
         for (int c = lane; c < p.chunks; c += 32) {
             const float4 f = p.stats[int64_t(c) * p.T + row];
-            Stats o;
-            o.m = f.x; o.s = f.y; o.d = f.z;
-            st.join(o);
+            Stats o{f.x, f.y, f.z};
+            o.raise(m);
+            st.s += o.s;
+            st.d += o.d;
         }
-        st = ib::score::warp_join(st);
+        st.s = ib::warp_sum(st.s);
+        st.d = ib::warp_sum(st.d);
         if (lane == 0) {
             total = st;
             const int token = p.tokens ? p.tokens[row] : -1;

@@ -19,8 +19,9 @@ using ib::score::Stats;
 using bf16 = __nv_bfloat16;
 
 // ------------------------------------------------------------------------------------------------ from logits
-// A row is shared by the CTAs of a cluster, each taking a contiguous slice. A thread takes every THREADS-th 16-byte unit, four at a time, and
-// the next four are requested before these are looked at; the statistics need no barrier until the end.
+// A row is shared by the CTAs of a cluster, each taking a contiguous slice of its 16-byte units (up to three elements before the first and behind
+// the last whole unit are the first CTA's beside them). A thread takes every THREADS-th unit, four at a time, and the next four are
+// requested before these are looked at; the statistics need no barrier until the end.
 // The alternatives cost the stream one comparison for four units (the thread's largest element and its id): the `top` best of all elements
 // lie with at most `top` threads, those whose largest reaches the top-th largest of the threads'.  A bound on that is enough: the top-th
 // of the largest of 64 groups of 8 threads.  The elements of the few threads that reach it are read again (from L2), those that
@@ -31,7 +32,7 @@ constexpr int THREADS = 512, UNITS = 4, GROUPS = THREADS / 8;
 constexpr int SEGMENT = 48;                                              // units of a thread in a segment
 constexpr int MAX_TOP = ib::score::MAX_TOP;
 constexpr int ROOM = 5120;                                               // keys of a segment's candidates
-static_assert(ROOM >= MAX_TOP * SEGMENT * 4 && SEGMENT % UNITS == 0 && MAX_TOP <= GROUPS, "the candidates fit");
+static_assert(ROOM >= MAX_TOP * SEGMENT * 4 + 6 + 8 * MAX_TOP && SEGMENT % UNITS == 0 && MAX_TOP <= GROUPS, "the candidates fit");
 
 struct Params {
     const float* logits;
@@ -65,6 +66,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 token_logprobs_kernel(const Params p) {
     extern __shared__ __align__(16) unsigned long long keys[];           // TOP: the list [MAX_TOP], candidates [ROOM], the new list [MAX_TOP]
     __shared__ Stats red[THREADS / 32];
+    __shared__ float red_m[THREADS / 32];
     __shared__ Stats parts[CL];                                           // of the cluster's CTAs, in the first
     __shared__ __align__(16) unsigned long long lists[TOP ? CL * MAX_TOP : 1];
     __shared__ unsigned long long best[TOP ? GROUPS : 1], bound;
@@ -73,11 +75,14 @@ token_logprobs_kernel(const Params p) {
     const int64_t b = blockIdx.x / CL;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float* row = p.logits + b * p.vocab;
-    // the row's first element sits `ahead` floats behind a 16-byte boundary: units are counted from that boundary
-    const int ahead = int((reinterpret_cast<uintptr_t>(row) >> 2) & 3);
-    const int64_t n_units = (p.vocab + ahead + 3) / 4;
+    // whole units start `lead` elements into the row
+    const int lead = int(min(int64_t((4 - ((reinterpret_cast<uintptr_t>(row) >> 2) & 3)) & 3), p.vocab));
+    const int64_t n_units = (p.vocab - lead) / 4;
+    const int edges = lead + int((p.vocab - lead) & 3);                   // elements outside of whole units
     const int64_t per = (n_units + CL - 1) / CL, u_lo = min(n_units, per * rank);
     const int mine = int(min(n_units, u_lo + per) - u_lo);                // units of this CTA
+    const float4* units = reinterpret_cast<const float4*>(row + lead) + u_lo;
+    const uint32_t id0 = uint32_t(lead + 4 * u_lo);                       // of this CTA's first unit's first element
     unsigned long long* found = keys + MAX_TOP;
     if (TOP) {
         if (threadIdx.x < MAX_TOP) keys[threadIdx.x] = keys[MAX_TOP + ROOM + threadIdx.x] = 0;
@@ -92,61 +97,58 @@ token_logprobs_kernel(const Params p) {
         token = p.tokens[b];
         if (token >= 0 && token < p.vocab) at = row[token];
     }
-    // unit i of this CTA: four elements, those outside the row as -inf
-    auto fetch = [&](int i) {
-        const int64_t e = 4 * (u_lo + i) - ahead;
-        float4 f;
-        if (i < mine && e >= 0 && e + 4 <= p.vocab) f = *reinterpret_cast<const float4*>(row + e);
-        else {
-            const bool in = i < mine;
-            f.x = in && e >= 0 && e < p.vocab ? row[e] : -INFINITY;
-            f.y = in && e + 1 >= 0 && e + 1 < p.vocab ? row[e + 1] : -INFINITY;
-            f.z = in && e + 2 >= 0 && e + 2 < p.vocab ? row[e + 2] : -INFINITY;
-            f.w = in && e + 3 < p.vocab ? row[e + 3] : -INFINITY;
-        }
-        return f;
-    };
-    auto id_of = [&](int i, int k) { return uint32_t(4 * (u_lo + i) - ahead + k); };
+    auto fetch = [&](int i) { return i < mine ? units[i] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY); };
     Stats st;
     st.clear();
     float4 next[UNITS];
 #pragma unroll
     for (int j = 0; j < UNITS; j++) next[j] = fetch(j * THREADS + int(threadIdx.x));
-    for (int s0 = 0; s0 < mine; s0 += SEGMENT * THREADS) {
+    if (rank == 0 && int(threadIdx.x) < edges) {
+        const int64_t e = int(threadIdx.x) < lead ? int64_t(threadIdx.x) : p.vocab - edges + threadIdx.x;
+        float z[1] = {row[e]};
+        if (TOP && z[0] > -INFINITY) found[atomicAdd(&n_keys, 1)] = ib::score::key(z[0], uint32_t(e));
+        if (p.cap > 0.0f) {
+            float l[1];
+            ib::score::cap_logits<1>(l, z, p.scale, p.cap);
+            st.add<1>(l, l[0]);
+        } else {
+            st.add<1>(z, z[0], p.scale);
+        }
+    }
+    int s0 = 0;
+    do {
         const int s1 = min(mine, s0 + SEGMENT * THREADS);
         float largest = -INFINITY;
-        int largest_at = 0;                                               // unit (in the CTA) x 4 + element
+        int largest_at = 0;                                               // element of this CTA's units
         for (int i0 = s0; i0 < s1; i0 += UNITS * THREADS) {
             float z[UNITS * 4];
 #pragma unroll
             for (int j = 0; j < UNITS; j++) { z[4 * j] = next[j].x; z[4 * j + 1] = next[j].y; z[4 * j + 2] = next[j].z; z[4 * j + 3] = next[j].w; }
 #pragma unroll
             for (int j = 0; j < UNITS; j++) next[j] = fetch(i0 + (UNITS + j) * THREADS + int(threadIdx.x));
-            if (TOP) {
-                float m = z[0];
+            const float m = ib::score::largest_of<UNITS * 4>(z);
+            if (TOP && m > largest) {
+                largest = m;
+                int which = 0;
 #pragma unroll
-                for (int i = 1; i < UNITS * 4; i++) m = fmaxf(m, z[i]);
-                if (m > largest) {
-                    largest = m;
-                    int which = 0;
-#pragma unroll
-                    for (int i = UNITS * 4 - 1; i >= 0; i--) which = z[i] == m ? i : which;
-                    largest_at = 4 * (i0 + (which >> 2) * THREADS + int(threadIdx.x)) + (which & 3);
-                }
+                for (int i = UNITS * 4 - 1; i >= 0; i--) which = z[i] == m ? i : which;
+                largest_at = 4 * (i0 + (which >> 2) * THREADS + int(threadIdx.x)) + (which & 3);
             }
             if (p.cap > 0.0f) {
                 float l[UNITS * 4];
                 ib::score::cap_logits<UNITS * 4>(l, z, p.scale, p.cap);
-                st.add<UNITS * 4>(l);
+                st.add<UNITS * 4>(l, ib::score::largest_of<UNITS * 4>(l));
             } else {
-                st.add<UNITS * 4>(z, p.scale);
+                st.add<UNITS * 4>(z, m, p.scale);
             }
         }
+        s0 += SEGMENT * THREADS;
         if (TOP) {
             const unsigned long long last = keys[p.top - 1];              // 0: fewer than top so far
-            const unsigned long long mine_best = largest > -INFINITY ? ib::score::key(largest, id_of(largest_at >> 2, largest_at & 3)) : 0;
+            const unsigned long long mine_best = largest > -INFINITY ? ib::score::key(largest, id0 + largest_at) : 0;
             bool in = mine_best > last;
-            if (__syncthreads_count(in) == 0) continue;
+            const int any = __syncthreads_count(in), held = n_keys;        // held: elements outside of whole units
+            if (any + held == 0) continue;
             unsigned long long g = mine_best;
 #pragma unroll
             for (int o = 4; o > 0; o >>= 1) {
@@ -165,28 +167,28 @@ token_logprobs_kernel(const Params p) {
             __syncthreads();
             unsigned long long least = max(bound, last + 1);
             in = mine_best >= least;
-            const int reach = (s1 - s0 + THREADS - 1) / THREADS;          // units of a thread
-            if (__syncthreads_count(in) * reach * 4 > ROOM) {
-                if (in) found[atomicAdd(&n_keys, 1)] = mine_best;
+            const int begin = s0 - SEGMENT * THREADS, reach = (s1 - begin + THREADS - 1) / THREADS;        // units of a thread
+            if (__syncthreads_count(in) * reach * 4 + held > ROOM) {
+                if (in) found[6 + atomicAdd(&n_keys, 1) - held] = mine_best;
                 __syncthreads();
-                ranked(found, n_keys, p.top, [&](int above, unsigned long long k) { if (above == p.top - 1) bound = k; });
+                ranked(found + 6, n_keys - held, p.top, [&](int above, unsigned long long k) { if (above == p.top - 1) bound = k; });
                 __syncthreads();
                 least = max(bound, last + 1);
                 in = mine_best >= least;
-                if (threadIdx.x == 0) n_keys = 0;
+                if (threadIdx.x == 0) n_keys = held;
                 __syncthreads();
             }
             // a warp reads its chosen threads' units again, a thread at a time
             for (uint32_t todo = __ballot_sync(0xffffffffu, in); todo; todo &= todo - 1) {
                 const int t = warp * 32 + __ffs(todo) - 1;
                 for (int j = lane; j < reach; j += 32) {
-                    const int i = s0 + j * THREADS + t;
+                    const int i = begin + j * THREADS + t;
                     if (i >= s1) break;
-                    const float4 f = fetch(i);
+                    const float4 f = units[i];
                     const float v[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        const unsigned long long key = v[k] > -INFINITY ? ib::score::key(v[k], id_of(i, k)) : 0;
+                        const unsigned long long key = v[k] > -INFINITY ? ib::score::key(v[k], id0 + 4 * i + k) : 0;
                         if (key >= least) found[atomicAdd(&n_keys, 1)] = key;
                     }
                 }
@@ -201,15 +203,20 @@ token_logprobs_kernel(const Params p) {
             if (threadIdx.x == 0) { n_keys = 0; bound = 0; }
             __syncthreads();
         }
-    }
+    } while (s0 < mine);
     ib::pdl_launch_dependents();
-    st = ib::score::warp_join(st);
+    // the block's maximum, each thread rescaled to it once, sums
+    const float warp_m = ib::warp_max(st.m);
+    if (lane == 0) red_m[warp] = warp_m;
+    __syncthreads();
+    st.raise(ib::warp_max(red_m[lane & (THREADS / 32 - 1)]));
+    st.s = ib::warp_sum(st.s);
+    st.d = ib::warp_sum(st.d);
     if (lane == 0) red[warp] = st;
     __syncthreads();
     if (warp == 0) {
-        st.clear();
-        if (lane < THREADS / 32) st = red[lane];
-        st = ib::score::warp_join(st);
+        st.s = ib::warp_sum(lane < THREADS / 32 ? red[lane].s : 0.0f);
+        st.d = ib::warp_sum(lane < THREADS / 32 ? red[lane].d : 0.0f);
     }
     if (CL > 1) {
         auto cluster = cg::this_cluster();
@@ -275,7 +282,7 @@ IB_EXPORT int ib_max_top_logprobs() { return MAX_TOP; }
 IB_EXPORT int ib_token_logprobs(const float* logits, int64_t rows, int64_t vocab, const int* tokens, int top, float scale, float cap, float* logprob,
                                 float* entropy, int* top_ids, float* top_logprobs, int cluster, int* status, cudaStream_t stream) {
     if (rows <= 0) return IB_OK;
-    if (vocab <= 0 || vocab >= 0x7fffffff) return ib::fail(IB_ERR_ARG, "token_logprobs: vocabulary %lld out of range", (long long)vocab);
+    if (vocab <= 0 || vocab >= (1LL << 30)) return ib::fail(IB_ERR_ARG, "token_logprobs: vocabulary %lld out of range", (long long)vocab);
     if (rows > 0x7fffffff / 8) return ib::fail(IB_ERR_ARG, "token_logprobs: too many rows (%lld)", (long long)rows);
     if (top < 0 || top > MAX_TOP) return ib::fail(IB_ERR_ARG, "token_logprobs: 0 to %d alternatives, not %d", MAX_TOP, top);
     if (!(scale > 0.0f) || !(cap >= 0.0f)) return ib::fail(IB_ERR_ARG, "token_logprobs: the scale must be positive, the cap not negative");

@@ -306,11 +306,6 @@ def linear_f32_tc(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor]
     return out
 
 
-@functools.lru_cache(maxsize=None)
-def sm_count(device: torch.device) -> int:
-    return torch.cuda.get_device_properties(device).multi_processor_count
-
-
 def head_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[torch.Tensor], top: int, scale: float, softcap: float,
                   status: Optional[torch.Tensor]):
     """``ops.head_logprobs`` (which has looked at the operands) without logits in memory; None for rows that the streaming product takes
@@ -319,12 +314,12 @@ def head_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[torch.Tenso
     T, H = x.shape
     if T <= skinny_limits()[0] or H % 8 or (x.data_ptr() & 15) or (w.data_ptr() & 15):
         return None
-    sms, nbytes = sm_count(x.device), c_int64()
+    sms, nbytes = ops.sm_count(x.device), c_int64()
     f = _fn("score_head", "ib_head_logprobs_scratch", [c_int64] * 3 + [c_int] * 2 + [c_void_p])
     if f(T, w.shape[0], H, top, sms, ctypes.byref(nbytes)) != 0:
         return None
-    r = ops._new_logprobs(T, top, x.device)
-    scratch = torch.empty(nbytes.value, dtype=torch.uint8, device=x.device)
+    r = ops._new_logprobs(T, top, x)
+    scratch = x.new_empty((nbytes.value,), dtype=torch.uint8)
     f = _fn("score_head", "ib_head_logprobs", [c_void_p] * 2 + [c_int64] * 3 + [c_void_p, c_int, c_float, c_float] + [c_void_p] * 5 + [c_int] + [c_void_p] * 2)
     _call(f, x.data_ptr(), w.data_ptr(), T, w.shape[0], H, _ptr(tokens), top, float(scale), float(softcap), r.logprob.data_ptr(),
           r.entropy.data_ptr(), r.top_ids.data_ptr(), r.top_logprobs.data_ptr(), scratch.data_ptr(), sms,

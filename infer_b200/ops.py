@@ -318,32 +318,39 @@ def max_top_logprobs() -> int:
     return int(_fn("score", "ib_max_top_logprobs", [])())
 
 
-def _check_logprobs(rows: int, device, tokens: Optional[torch.Tensor], top: int, scale: float, softcap: float, status: Optional[torch.Tensor]) -> int:
-    top = int(top)
+def _check_logprobs(rows: int, device, tokens: Optional[torch.Tensor], status: Optional[torch.Tensor]) -> None:
+    for name, t, n in (("tokens", tokens, rows), ("status", status, 1)):
+        if t is None:
+            continue
+        if not t.is_cuda or t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+            _check(t, name, torch.int32, (n,))
+        if t.device != device:
+            raise KernelError(f"{name} must lie on {device}, not on {t.device}")
+
+
+def _check_distribution(top: int, scale: float, softcap: float) -> None:
     if not 0 <= top <= max_top_logprobs():
         raise KernelError(f"0 to {max_top_logprobs()} alternatives can be asked for, not {top}")
-    if not (scale > 0 and math.isfinite(scale)):
+    if not (0 < scale < math.inf):
         raise KernelError(f"the logits' scale must be positive and finite, not {scale}")
-    if not (softcap >= 0 and math.isfinite(softcap)):
+    if not (0 <= softcap < math.inf):
         raise KernelError(f"the logits' cap must be positive and finite, or 0 for none, not {softcap}")
-    for name, t, shape in (("tokens", tokens, (rows,)), ("status", status, (1,))):
-        if t is not None:
-            _check(t, name, torch.int32, shape)
-            if t.device != device:
-                raise KernelError(f"{name} must lie on {device}, not on {t.device}")
-    return top
 
 
-def _new_logprobs(rows: int, top: int, device) -> TokenLogprobs:
-    both = torch.empty((2, rows), dtype=torch.float32, device=device)
-    return TokenLogprobs(both[0], both[1], torch.empty((rows, top), dtype=torch.int32, device=device),
-                         torch.empty((rows, top), dtype=torch.float32, device=device))
+def _new_logprobs(rows: int, top: int, like: torch.Tensor) -> TokenLogprobs:
+    """Results on the device of ``like``. (new_empty: half a microsecond less than empty, four times a call.)"""
+    f32 = torch.float32
+    return TokenLogprobs(like.new_empty((rows,), dtype=f32), like.new_empty((rows,), dtype=f32),
+                         like.new_empty((rows, top), dtype=torch.int32), like.new_empty((rows, top), dtype=f32))
 
 
 def _logprobs_cluster(rows: int, vocab: int, sm_count: int) -> int:
-    """CTAs that share a row of logits: while the rows alone leave the GPU idle, and each keeps a chunk of 8,192 elements."""
-    cluster = 8
-    while cluster > 1 and (rows * cluster > 4 * sm_count or vocab < 8192 * cluster // 2):
+    """CTAs that share a row of logits: as many as leave all rows running at once (two CTAs an SM; clusters of eight do not fit everywhere
+    and get one), and each some 4,000 elements. (64 rows x 151,936, 20 alternatives, clusters of 8, 4, 2, 1: 41, 24, 29, 32 us.)"""
+    if 8 * rows <= sm_count and vocab > 16384:
+        return 8
+    cluster = 4
+    while cluster > 1 and (rows * cluster > 2 * sm_count or vocab < 4096 * cluster // 2):
         cluster //= 2
     return cluster
 
@@ -358,20 +365,31 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     [0, V): NaN, and the status word (if given) is set to 1. ``scale`` / ``softcap``: the distribution is that of
     softcap * tanh(logits * scale / softcap) (-inf stays -inf), or logits * scale without a cap; alternatives go by ``logits``.
     Each call may run on any stream; a captured one reads its inputs anew at each replay."""
+    _check_distribution(top, scale, softcap)
     _check(logits, "logits", torch.float32)
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise KernelError(f"logits must be [rows, vocabulary], got {tuple(logits.shape)}")
     T, V = logits.shape
-    top = _check_logprobs(T, logits.device, tokens, top, scale, softcap, status)
-    r = _new_logprobs(T, top, logits.device) if out is None else out
+    device = logits.device
+    if device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return token_logprobs(logits, tokens, top, status, scale, softcap, out)
+    _check_logprobs(T, device, tokens, status)
+    r = _new_logprobs(T, top, logits) if out is None else out
     if T == 0:
         return r
-    from . import fast_ops
-    f = _fn("score", "ib_token_logprobs", [c_void_p, c_int64, c_int64, c_void_p, c_int, c_float, c_float] + [c_void_p] * 4 + [c_int] + [c_void_p] * 2)
-    with torch.cuda.device(logits.device):
-        _call(f, logits.data_ptr(), T, V, _ptr(tokens), top, float(scale), float(softcap), r.logprob.data_ptr(), r.entropy.data_ptr(),
-              r.top_ids.data_ptr(), r.top_logprobs.data_ptr(), _logprobs_cluster(T, V, fast_ops.sm_count(logits.device)), _ptr(status), _stream())
+    f = _fn("score", "ib_token_logprobs", _TOKEN_LOGPROBS_ARGS)
+    _call(f, logits.data_ptr(), T, V, _ptr(tokens), top, scale, softcap, r.logprob.data_ptr(), r.entropy.data_ptr(),
+          r.top_ids.data_ptr(), r.top_logprobs.data_ptr(), _logprobs_cluster(T, V, sm_count(device)), _ptr(status), _stream())
     return r
+
+
+_TOKEN_LOGPROBS_ARGS = [c_void_p, c_int64, c_int64, c_void_p, c_int, c_float, c_float] + [c_void_p] * 4 + [c_int] + [c_void_p] * 2
+
+
+@functools.lru_cache(maxsize=None)
+def sm_count(device: torch.device) -> int:
+    return torch.cuda.get_device_properties(device).multi_processor_count
 
 
 def head_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0, scale: float = 1.0,
@@ -380,31 +398,39 @@ def head_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[torch.Tenso
     not kept: bfloat16 rows go through a kernel that holds them in tensor memory only; up to 16 rows, rows that do not keep to 16 bytes and
     float32 go through logits of a few rows at a time. ``w`` is a loaded weight (as for ``linear``). A kernel whose bounded wait runs out
     says so in the device's status word."""
+    _check_distribution(top, scale, softcap)
+    _check_product("head_logprobs", x, w)
+    (T, K), V, device = x.shape, w.shape[0], x.device
+    if device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return head_logprobs(x, w, tokens, top, scale, softcap, status)
+    _check_logprobs(T, device, tokens, status)
+    from . import fast_ops
+    if T > 0 and x.dtype is torch.bfloat16:
+        r = fast_ops.head_logprobs(x, w, tokens, top, scale, softcap, status)
+        if r is not None:
+            return r
+    r = _new_logprobs(T, top, x)
+    step = max(1, min(T, HEAD_LOGITS // V))
+    logits = x.new_empty((step, V), dtype=torch.float32)
+    for lo in range(0, T, step):
+        hi = min(T, lo + step)
+        z, rows, part, here = (logits, x, r, tokens) if step == T else \
+            (logits[:hi - lo], x[lo:hi], TokenLogprobs(*(t[lo:hi] for t in r)), None if tokens is None else tokens[lo:hi])
+        if fast_ops.linear(rows, w, None, None, torch.float32, z) is None:
+            linear_plain(rows, w, out=z, w_ready=True)
+        token_logprobs(z, here, top, status, scale, softcap, part)
+    return r
+
+
+def _check_product(what: str, x: torch.Tensor, w: torch.Tensor) -> None:
     _check(x, "x")
     _check(w, "w", x.dtype)
     dtype_code(x.dtype)
-    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or min(w.shape) < 1:
-        raise KernelError(f"head_logprobs: x is {tuple(x.shape)} but w is {tuple(w.shape)}")
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or 0 in w.shape:
+        raise KernelError(f"{what}: x is {tuple(x.shape)} but w is {tuple(w.shape)}")
     if w.device != x.device:
         raise KernelError(f"w must lie on {x.device}, not on {w.device}")
-    T, V = x.shape[0], w.shape[0]
-    top = _check_logprobs(T, x.device, tokens, top, scale, softcap, status)
-    from . import fast_ops
-    with torch.cuda.device(x.device):
-        if T > 0 and x.dtype == torch.bfloat16:
-            r = fast_ops.head_logprobs(x, w, tokens, top, scale, softcap, status)
-            if r is not None:
-                return r
-        r = _new_logprobs(T, top, x.device)
-        step = max(1, min(T, HEAD_LOGITS // V))
-        logits = torch.empty((step, V), dtype=torch.float32, device=x.device)
-        for lo in range(0, T, step):
-            hi = min(T, lo + step)
-            z = logits[:hi - lo]
-            if fast_ops.linear(x[lo:hi], w, None, None, torch.float32, z) is None:
-                linear_plain(x[lo:hi], w, out=z, w_ready=True)
-            token_logprobs(z, None if tokens is None else tokens[lo:hi], top, status, scale, softcap, TokenLogprobs(*(t[lo:hi] for t in r)))
-    return r
 
 
 # Elements of the logits that ``head_logprobs`` has in memory at a time where it needs them: 64 MB, which stay in L2.
@@ -420,14 +446,10 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
     (0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3)))), "gelu" (0.5 z (1 + erf(z / sqrt 2))), "silu" (z / (1 + e^-z)). The result is
     float32 or bfloat16 (default: as x; with a residual float32). ``w`` is a loaded weight (as for ``linear``). A kernel whose bounded wait
     runs out says so in the device's status word."""
-    _check(x, "x")
-    _check(w, "w", x.dtype)
-    dtype_code(x.dtype)
-    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or min(w.shape) < 1:
-        raise KernelError(f"linear_act: x is {tuple(x.shape)} but w is {tuple(w.shape)}")
     if activation not in ACTIVATIONS:
         raise KernelError(f"activation {activation!r} is not among {sorted(ACTIVATIONS)}")
-    (M, K), N = x.shape, w.shape[0]
+    _check_product("linear_act", x, w)
+    (M, K), N, device = x.shape, w.shape[0], x.device
     if bias is not None:
         _check(bias, "bias", torch.float32, (N,))
     if residual is not None:
@@ -437,20 +459,22 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
     dtype_code(out_dtype)
     if out is not None:
         _check(out, "out", out_dtype, (M, N))
-    for name, t in (("w", w), ("bias", bias), ("residual", residual), ("out", out)):
-        if t is not None and t.device != x.device:
-            raise KernelError(f"{name} must lie on {x.device}, not on {t.device}")
-    with torch.cuda.device(x.device):
-        if out is None:
-            out = torch.empty((M, N), dtype=out_dtype, device=x.device)
-        if out.numel() == 0:
-            return out
-        from . import fast_ops
-        z = fast_ops.linear(x, w, bias, None, torch.float32, None)
-        if z is None:
-            z = linear_plain(x, w, bias, None, torch.float32, w_ready=True)
-        f = _fn("score", "ib_act_residual", [c_void_p] * 3 + [c_int64, c_int, c_int, c_void_p])
-        _call(f, z.data_ptr(), _ptr(residual), out.data_ptr(), M * N, ACTIVATIONS[activation], dtype_code(out_dtype), _stream())
+    for name, t in (("bias", bias), ("residual", residual), ("out", out)):
+        if t is not None and t.device != device:
+            raise KernelError(f"{name} must lie on {device}, not on {t.device}")
+    if device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return linear_act(x, w, bias, activation, residual, out_dtype, out)
+    if out is None:
+        out = x.new_empty((M, N), dtype=out_dtype)
+    if M == 0:
+        return out
+    from . import fast_ops
+    z = fast_ops.linear(x, w, bias, None, torch.float32, None)
+    if z is None:
+        z = linear_plain(x, w, bias, None, torch.float32, w_ready=True)
+    f = _fn("score", "ib_act_residual", [c_void_p] * 3 + [c_int64, c_int, c_int, c_void_p])
+    _call(f, z.data_ptr(), _ptr(residual), out.data_ptr(), M * N, ACTIVATIONS[activation], dtype_code(out_dtype), _stream())
     return out
 
 
