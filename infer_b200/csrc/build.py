@@ -57,7 +57,8 @@ DEFAULT_DEFINES = {"attn": {"IB_HEAD_DIM": 128}, "attn_tc": {"IB_HEAD_DIM": 128}
 
 
 # a second form of a module that a model uses beside the first (built by build_all() too)
-MORE_DEFINES = {"attn_tc": {"IB_HEAD_DIM": 128, "IB_ATTN_BN": 128}}
+MORE_DEFINES = {"attn_tc": {"IB_HEAD_DIM": 128, "IB_ATTN_BN": 128}, "gemm": {"IB_ACT": 1}, "lin32": {"IB_ACT": 1},
+                "lin32_tc": {"IB_ACT": 1}}
 
 
 class BuildError(RuntimeError):

@@ -45,6 +45,15 @@
 #include <mutex>
 #include <unordered_map>
 
+// Compiled with IB_ACT the same kernels put an activation between bias and residual (a library of its own: the products without one stay
+// as they are).
+#ifdef IB_ACT
+#include "score.cuh"
+#define IB_ACTIVATE_ALL(p, x) ib::score::activate_all<16>(x, (p).act)
+#else
+#define IB_ACTIVATE_ALL(p, x) do {} while (0)
+#endif
+
 IB_DEFINE_LAST_ERROR()
 
 namespace {
@@ -207,6 +216,9 @@ struct GemmParams {
     // and which first k a tile's expert has: row (tn / g_tph) * g_half + expert * g_rows + (tn % g_tph) * width, k = expert * g_k
     const int* tiles;
     int g_tiles_n, g_tph, g_half, g_rows, g_k;
+#ifdef IB_ACT
+    int act;
+#endif
 };
 
 template <int BN> struct Cfg {
@@ -293,10 +305,14 @@ __device__ __forceinline__ void epilogue_store(const GemmParams& p, const float*
             const int64_t m = b_row0 + j;
             res[j] = (p.residual && m < p.M && j < ncols) ? p.residual[m * p.N + n] : 0.0f;
         }
+        float x[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) x[j] = v[j] + b;
+        IB_ACTIVATE_ALL(p, x);
 #pragma unroll
         for (int j = 0; j < 16; j++) {
             const int64_t m = b_row0 + j;
-            if (m < p.M && j < ncols) store_elem<TOut>(out + m * p.N + n, v[j] + b + res[j]);
+            if (m < p.M && j < ncols) store_elem<TOut>(out + m * p.N + n, x[j] + res[j]);
         }
     } else {
         const int64_t m = a_row;
@@ -306,6 +322,7 @@ __device__ __forceinline__ void epilogue_store(const GemmParams& p, const float*
             float x[16];
 #pragma unroll
             for (int j = 0; j < 16; j++) x[j] = v[j] + (p.bias ? p.bias[n0 + j] : 0.0f);
+            IB_ACTIVATE_ALL(p, x);
             if (p.residual) {
                 const float4* r4 = reinterpret_cast<const float4*>(p.residual + m * p.N + n0);
 #pragma unroll
@@ -334,13 +351,16 @@ __device__ __forceinline__ void epilogue_store(const GemmParams& p, const float*
                 }
             }
         } else {
+            float x[16];
+#pragma unroll
+            for (int j = 0; j < 16; j++) x[j] = v[j] + (p.bias && n0 + j < p.N ? p.bias[n0 + j] : 0.0f);
+            IB_ACTIVATE_ALL(p, x);
 #pragma unroll
             for (int j = 0; j < 16; j++) {
                 const int64_t n = n0 + j;
                 if (n < p.N && j < ncols) {
-                    float x = v[j] + (p.bias ? p.bias[n] : 0.0f);
-                    if (p.residual) x += p.residual[m * p.N + n];
-                    store_elem<TOut>(out + m * p.N + n, x);
+                    if (p.residual) x[j] += p.residual[m * p.N + n];
+                    store_elem<TOut>(out + m * p.N + n, x[j]);
                 }
             }
         }
@@ -652,8 +672,11 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__
                     if (a_row < p.N) {
                         TOut* dst = reinterpret_cast<TOut*>(p.out) + (int64_t(tile_b) * BN + c0) * p.N + a_row;
 #pragma unroll
+                        for (int j = 0; j < 16; j++) v[j] += own_bias;
+                        IB_ACTIVATE_ALL(p, v);
+#pragma unroll
                         for (int j = 0; j < 16; j++)
-                            if (j < ncols && int64_t(tile_b) * BN + c0 + j < p.M) store_elem<TOut>(dst + j * p.N, v[j] + own_bias + own_res[j]);
+                            if (j < ncols && int64_t(tile_b) * BN + c0 + j < p.M) store_elem<TOut>(dst + j * p.N, v[j] + own_res[j]);
                     }
                 } else {
                     epilogue_store<TOut>(p, v, a_row, int64_t(tile_b) * BN + c0, ncols);
@@ -1330,10 +1353,18 @@ IB_EXPORT int ib_gemm_tc(const void* x, const void* w, const float* bias, const 
         bn = 256;
     } else if (bn >= 256 && (swap || splits > 1)) return ib::fail(IB_ERR_ARG, "gemm_tc: the persistent kernel takes the plain mapping without K slices");
     if (!status) return ib::fail(IB_ERR_ARG, "gemm_tc: a status word is required");
+#ifdef IB_ACT
+    const int act = epi;                                          // (the library with activations has no other epilogues)
+    if (act < 0 || act >= ib::score::ACTIVATIONS) return ib::fail(IB_ERR_ARG, "gemm_tc: unknown activation %d", act);
+    epi = 0;
+#endif
     if (epi != 0 && epi != 2) return ib::fail(IB_ERR_ARG, "gemm_tc: unknown epilogue %d", epi);
     if (epi == 2 && (N % 16 || bias || residual)) return ib::fail(IB_ERR_ARG, "gemm_tc: the SwiGLU epilogue needs N %% 16 == 0 and no bias or residual");
     GemmParams p = {};
     p.epi = epi;
+#ifdef IB_ACT
+    p.act = act;
+#endif
     p.swap = swap ? 1 : 0;
     p.M = M; p.N = N; p.K = K;
     p.rows_a = swap ? N : M;
@@ -1405,6 +1436,7 @@ IB_EXPORT int ib_gemm_tc(const void* x, const void* w, const float* bias, const 
     }
 }
 
+#ifndef IB_ACT
 // A product whose rows are grouped by expert (expert_ops.cu): x [max_tiles * 128, K] bfloat16, a whole number of 128-row tiles an
 // expert, tiles [0] = the tiles in use and tiles[1 + i] the expert of tile i, in device memory. w bfloat16 is one matrix for all
 // experts. side 0 (an expert's rows of a stack of `halves` matrices [experts * n_expert, K]): out [rows, halves * padded],
@@ -1538,3 +1570,4 @@ IB_EXPORT int ib_gemm_tc_trace(long long* host) {
     return cudaMemcpyFromSymbol(host, ib_gemm_trace, sizeof(ib_gemm_trace)) == cudaSuccess ? IB_OK : IB_ERR_CUDA;
 }
 #endif
+#endif  // IB_ACT

@@ -31,6 +31,7 @@
 // 16b+8..16b+15 = the matching up features): out[m, 8b + r] = silu(gate) * up, bfloat16 [M, N/2].
 // K must be a multiple of 8 (16-byte alignment of every row); anything else is refused.
 #include "common.cuh"
+#include "score.cuh"
 
 #include <cooperative_groups.h>
 
@@ -139,6 +140,7 @@ struct GemvParams {
     int n_stages, per_cta;    // stages of a tile's K, and of a CTA of its cluster
     int groups;               // tile walkers in the grid (grid = groups * cluster); a walker takes every groups-th tile
     int* status;
+    int act;                  // EPI 3: the activation between bias and residual
 };
 
 template <int NT, int EPI, typename TOut, bool NWS>
@@ -450,6 +452,10 @@ bulk_gemv_kernel(const GemvParams p) {
             if (n < N) {
                 if (p.bias) v += p.bias[n];
                 if constexpr (EPI == 1) v += p.residual[int64_t(m) * N + n];
+                if constexpr (EPI == 3) {
+                    v = ib::score::activate(v, p.act);
+                    if (p.residual) v += p.residual[int64_t(m) * N + n];
+                }
                 out[int64_t(m) * N + n] = ib::from_f32<TOut>(v);
             }
         }
@@ -480,6 +486,10 @@ int launch(const GemvParams& p, int out_dtype, int epi, int grid_ctas, cudaStrea
     if (epi == 1) {
         if (out_dtype != IB_F32 || !p.residual) return ib::fail(IB_ERR_ARG, "linear_skinny_bulk: the residual epilogue needs a float residual and output");
         IB_GEMV_LAUNCH(1, float);
+    }
+    if (epi == 3) {
+        if (out_dtype == IB_F32) IB_GEMV_LAUNCH_(3, float, false);
+        if (out_dtype == IB_BF16) IB_GEMV_LAUNCH_(3, bf16, false);
     }
     if (out_dtype == IB_F32) IB_GEMV_LAUNCH(0, float);
     if (out_dtype == IB_BF16) IB_GEMV_LAUNCH(0, bf16);
@@ -527,9 +537,9 @@ IB_EXPORT int ib_linear_skinny_bulk_limits(int* max_rows, int* max_fused_norm_k)
     return IB_OK;
 }
 
-IB_EXPORT int ib_linear_skinny_bulk(const void* x, const float* norm_w, float norm_eps, const void* w, const float* bias, const float* residual, void* out,
-                                    int64_t M, int64_t N, int64_t K, int out_dtype, int epi, int cluster, int sm_count,
-                                    int* status, cudaStream_t stream) {
+static int linear_skinny_bulk(const void* x, const float* norm_w, float norm_eps, const void* w, const float* bias, const float* residual, void* out,
+                              int64_t M, int64_t N, int64_t K, int out_dtype, int epi, int act, int cluster, int sm_count,
+                              int* status, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return IB_OK;
     if (M > 16) return ib::fail(IB_ERR_ARG, "linear_skinny_bulk: at most 16 rows, got %lld", (long long)M);
     if (K <= 0 || K % 8) return ib::fail(IB_ERR_ARG, "linear_skinny_bulk: K = %lld must be a positive multiple of 8", (long long)K);
@@ -551,10 +561,25 @@ IB_EXPORT int ib_linear_skinny_bulk(const void* x, const float* norm_w, float no
     // gate the ring's second slot where the whole GPU's rings fill at once (a CTA per half SM) and a tile is one stage
     p.gate_ring = (d.n_stages == 1 && d.cluster == 1 && tiles >= 2LL * sms) ? 1 : 0;
     p.nw_smem = norm_w ? 1 : 0;
+    p.act = act;
     p.groups = d.groups;
     const int grid_ctas = d.groups * d.cluster;
     if (M <= 8) return launch<1>(p, out_dtype, epi, grid_ctas, stream);
     return launch<2>(p, out_dtype, epi, grid_ctas, stream);
+}
+
+IB_EXPORT int ib_linear_skinny_bulk(const void* x, const float* norm_w, float norm_eps, const void* w, const float* bias, const float* residual, void* out,
+                                    int64_t M, int64_t N, int64_t K, int out_dtype, int epi, int cluster, int sm_count,
+                                    int* status, cudaStream_t stream) {
+    if (epi < 0 || epi > 2) return ib::fail(IB_ERR_ARG, "linear_skinny_bulk: unknown epilogue %d", epi);
+    return linear_skinny_bulk(x, norm_w, norm_eps, w, bias, residual, out, M, N, K, out_dtype, epi, 0, cluster, sm_count, status, stream);
+}
+
+// out = residual + act(x . w^T + bias), bias and residual or none, float or bfloat16 [M, N]; act: an activation's number (score.cuh).
+IB_EXPORT int ib_linear_skinny_act(const void* x, const void* w, const float* bias, const float* residual, void* out, int64_t M, int64_t N, int64_t K,
+                                   int out_dtype, int act, int sm_count, int* status, cudaStream_t stream) {
+    if (act < 0 || act >= ib::score::ACTIVATIONS) return ib::fail(IB_ERR_ARG, "linear_skinny_act: unknown activation %d", act);
+    return linear_skinny_bulk(x, nullptr, 0.0f, w, bias, residual, out, M, N, K, out_dtype, 3, act, 0, sm_count, status, stream);
 }
 
 #ifdef IB_GEMV_TRACE

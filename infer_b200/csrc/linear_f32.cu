@@ -24,6 +24,18 @@
 // where those would leave SMs idle.
 #include "common.cuh"
 
+// Compiled with IB_ACT the same kernels put an activation between bias and residual (a library of its own).
+#ifdef IB_ACT
+#include "score.cuh"
+#define IB_ACT_PARAM , int act
+#define IB_ACT_OF(a) , (a).act
+#define IB_ACT_ARG , act
+#else
+#define IB_ACT_PARAM
+#define IB_ACT_OF(a)
+#define IB_ACT_ARG
+#endif
+
 IB_DEFINE_LAST_ERROR()
 
 namespace {
@@ -68,8 +80,11 @@ __device__ __forceinline__ void lds_pairs(pair& a, pair& b, const float* at) {
     a = v.x; b = v.y;
 }
 
-__device__ __forceinline__ void store_result(float v, int64_t m, int64_t n, int64_t N, const float* bias, const float* residual, float* out) {
+__device__ __forceinline__ void store_result(float v, int64_t m, int64_t n, int64_t N, const float* bias, const float* residual, float* out IB_ACT_PARAM) {
     if (bias) v += bias[n];
+#ifdef IB_ACT
+    v = ib::score::activate(v, act);
+#endif
     if (residual) v += residual[m * N + n];
     out[m * N + n] = v;
 }
@@ -83,7 +98,7 @@ constexpr int gemv_smem() { return GSTAGES * (ROWS + MT) * GK * 4; }
 template <int ROWS, int MT, bool VEC>
 __global__ void __launch_bounds__(ROWS * GBLOCKS)
 gemv32_kernel(const float* __restrict__ x, const float* __restrict__ w, const float* __restrict__ bias, const float* residual,
-              float* out, int M, int64_t N, int64_t K, int w_ready) {
+              float* out, int M, int64_t N, int64_t K, int w_ready IB_ACT_PARAM) {
     extern __shared__ __align__(128) float stages[];           // [GSTAGES][ROWS rows of w, MT rows of x][GK]
     constexpr int THREADS = ROWS * GBLOCKS, UNITS = GK / 4;
     __shared__ float sums[THREADS / 32][4][GBLOCKS][MT + 1];   // per warp: 4 features x 8 blocks x rows
@@ -153,7 +168,7 @@ gemv32_kernel(const float* __restrict__ x, const float* __restrict__ w, const fl
     }
     wait_groups<0>();
     const int64_t n = n0 + feature;
-    if (blk < MT && blk < M && n < N) store_result(total, blk, n, N, bias, residual, out);
+    if (blk < MT && blk < M && n < N) store_result(total, blk, n, N, bias, residual, out IB_ACT_ARG);
 }
 
 // ------------------------------------------------------------------------------------------------ more rows
@@ -166,7 +181,7 @@ constexpr int tile_smem() { return TSTAGES * (8 * TM + 16 * TN) * PITCH * 4; }
 template <int TM, int TN, bool VEC>
 __global__ void __launch_bounds__(128, TM * TN > 16 ? 3 : 4)
 tile32_kernel(const float* __restrict__ x, const float* __restrict__ w, const float* __restrict__ bias, const float* residual,
-              float* out, int64_t M, int64_t N, int64_t K) {
+              float* out, int64_t M, int64_t N, int64_t K IB_ACT_PARAM) {
     extern __shared__ __align__(128) float stages[];           // [TSTAGES][BM rows of x, BN rows of w][PITCH]
     constexpr int BM = 8 * TM, BN = 16 * TN, UNITS = BLOCK_K / 4;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -233,7 +248,7 @@ tile32_kernel(const float* __restrict__ x, const float* __restrict__ w, const fl
 #pragma unroll
         for (int j = 0; j < TN; j++) {
             const int64_t n = n0 + tx + 8 * j;
-            if (m < M && n < N) store_result(total[i][j], m, n, N, bias, residual, out);
+            if (m < M && n < N) store_result(total[i][j], m, n, N, bias, residual, out IB_ACT_ARG);
         }
     }
 }
@@ -243,6 +258,9 @@ struct Args {
     float* out;
     int64_t M, N, K;
     int w_ready;
+#ifdef IB_ACT
+    int act;
+#endif
 };
 
 template <int ROWS, int MT, bool VEC>
@@ -250,7 +268,7 @@ int launch_gemv(const Args& a, cudaStream_t stream) {
     static ib::PerDevice allowed;
     if (const int rc = ib::allow_smem(allowed, "linear_f32", gemv32_kernel<ROWS, MT, VEC>, gemv_smem<ROWS, MT>())) return rc;
     return ib::launch("linear_f32", gemv32_kernel<ROWS, MT, VEC>, dim3(unsigned((a.N + ROWS - 1) / ROWS)), dim3(ROWS * GBLOCKS),
-                      size_t(gemv_smem<ROWS, MT>()), stream, 1u, a.x, a.w, a.bias, a.residual, a.out, int(a.M), a.N, a.K, a.w_ready);
+                      size_t(gemv_smem<ROWS, MT>()), stream, 1u, a.x, a.w, a.bias, a.residual, a.out, int(a.M), a.N, a.K, a.w_ready IB_ACT_OF(a));
 }
 
 template <int ROWS, bool VEC>
@@ -268,7 +286,7 @@ int launch_tile(const Args& a, cudaStream_t stream) {
     const dim3 grid{unsigned((a.N + 16 * TN - 1) / (16 * TN)), unsigned((a.M + 8 * TM - 1) / (8 * TM)), 1u};
     if (grid.y > 65535) return ib::fail(IB_ERR_ARG, "linear_f32: too many rows (%lld)", (long long)a.M);
     return ib::launch("linear_f32", tile32_kernel<TM, TN, VEC>, grid, dim3(128), size_t(tile_smem<TM, TN>()), stream, 1u, a.x, a.w, a.bias,
-                      a.residual, a.out, a.M, a.N, a.K);
+                      a.residual, a.out, a.M, a.N, a.K IB_ACT_OF(a));
 }
 
 template <bool VEC>
@@ -310,12 +328,12 @@ int dispatch(const Args& a, int kind, int sms, cudaStream_t stream) {
 // Every kind gives the same bits. residual may be out. w_ready: 1 = no kernel that may still run writes w (it may be read before
 // this kernel's predecessor has ended), 0 = w may come from the predecessor.
 IB_EXPORT int ib_linear_f32(const float* x, const float* w, const float* bias, const float* residual, float* out, int64_t M, int64_t N,
-                            int64_t K, int kind, int sm_count, int w_ready, cudaStream_t stream) {
+                            int64_t K, int kind, int sm_count, int w_ready IB_ACT_PARAM, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return IB_OK;
     if (K <= 0) return ib::fail(IB_ERR_ARG, "linear_f32: K must be positive");
     const int64_t lim = 1LL << 31;                             // of the blocks of 32 elements of K, and of CTAs with 8 features each
     if (N >= 8 * lim || K >= BLOCK_K * lim) return ib::fail(IB_ERR_ARG, "linear_f32: more features or columns than the kernels count");
-    const Args a{x, w, bias, residual, out, M, N, K, w_ready};
+    const Args a{x, w, bias, residual, out, M, N, K, w_ready IB_ACT_ARG};
     const int sms = sm_count > 0 ? sm_count : 148;
     const bool vec = K % 4 == 0 && ((uintptr_t(x) | uintptr_t(w)) & 15) == 0;
     return vec ? dispatch<true>(a, kind, sms, stream) : dispatch<false>(a, kind, sms, stream);

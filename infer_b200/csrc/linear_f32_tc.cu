@@ -35,6 +35,14 @@
 #include "common.cuh"
 #include "tc_ops.cuh"
 
+// Compiled with IB_ACT the same kernel puts an activation between bias and residual (a library of its own, which takes smaller matrices too).
+#ifdef IB_ACT
+#include "score.cuh"
+#define IB_ACTIVATE(p, v) ib::score::activate((v), (p).act)
+#else
+#define IB_ACTIVATE(p, v) (v)
+#endif
+
 IB_DEFINE_LAST_ERROR()
 
 namespace {
@@ -142,6 +150,9 @@ struct Params {
     int share;                                   // CTAs of a tile (a cluster)
     int* status;
     int w_ready;
+#ifdef IB_ACT
+    int act;
+#endif
 };
 
 __device__ __forceinline__ uint32_t map_cluster(uint32_t local_smem, uint32_t rank) {
@@ -423,6 +434,7 @@ linear32_tc_kernel(const Params p) {
                         continue;
                     }
                     if (p.bias) v += bias;
+                    v = IB_ACTIVATE(p, v);
                     if (p.residual) v += res[i];
                     p.out[m * p.N + n] = v;
                 }
@@ -465,6 +477,7 @@ linear32_tc_kernel(const Params p) {
             }
             if (mine) {
                 if (p.bias) v += p.bias[nf];
+                v = IB_ACTIVATE(p, v);
                 if (p.residual) v += p.residual[m * p.N + nf];
                 p.out[m * p.N + nf] = v;
             }
@@ -530,17 +543,29 @@ int launch_nt(const Params& p, const Plan& q, cudaStream_t stream) {
 
 // 1 where this kernel takes the matrix: a matter of N and K alone, so that every batch of rows takes the same way.
 IB_EXPORT int ib_linear_f32_tc_takes(int64_t N, int64_t K) {
+#ifdef IB_ACT
+    return N >= BM && K >= 2 * BK && N <= 65535LL * BM && K < (1LL << 31) ? 1 : 0;
+#else
     return N >= 1024 && K >= 1024 && N <= 65535LL * BM && K < (1LL << 31) ? 1 : 0;
+#endif
 }
 
 // residual may be out. w_ready: as in ib_linear_f32.
 IB_EXPORT int ib_linear_f32_tc(const float* x, const float* w, const float* bias, const float* residual, float* out, int64_t M, int64_t N,
-                               int64_t K, int sm_count, int w_ready, int* status, cudaStream_t stream) {
+                               int64_t K, int sm_count, int w_ready,
+#ifdef IB_ACT
+                               int act,
+#endif
+                               int* status, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return IB_OK;
     if (!ib_linear_f32_tc_takes(N, K)) return ib::fail(IB_ERR_ARG, "linear_f32_tc: a matrix of %lld x %lld is not taken", (long long)N, (long long)K);
     if (!status) return ib::fail(IB_ERR_ARG, "linear_f32_tc: a status word is required");
     const Plan q = make_plan(M, N, K, sm_count > 0 ? sm_count : 148);
-    const Params p{x, w, bias, residual, out, M, N, K, int((K + BK - 1) / BK), q.groups, q.groups / q.share, q.share, status, w_ready};
+    const Params p{x, w, bias, residual, out, M, N, K, int((K + BK - 1) / BK), q.groups, q.groups / q.share, q.share, status, w_ready
+#ifdef IB_ACT
+                   , act
+#endif
+    };
     const bool vec = K % 4 == 0 && ((uintptr_t(x) | uintptr_t(w)) & 15) == 0;
     return vec ? launch_nt<true>(p, q, stream) : launch_nt<false>(p, q, stream);
 }

@@ -136,6 +136,12 @@ __device__ __forceinline__ float activate(float z, int act) {
     }
     return z;
 }
+// N elements under one switch (a switch for each cost the epilogues more than the activations).
+template <int N> __device__ __forceinline__ void activate_all(float (&z)[N], int act) {
+#define IB_EACH(A) case A: { _Pragma("unroll") for (int i = 0; i < N; i++) z[i] = activate(z[i], A); break; }
+    switch (act) { IB_EACH(RELU) IB_EACH(RELU_SQUARED) IB_EACH(GELU_TANH) IB_EACH(GELU) IB_EACH(SILU) }
+#undef IB_EACH
+}
 
 }  // namespace score
 }  // namespace ib

@@ -306,6 +306,64 @@ def linear_f32_tc(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor]
     return out
 
 
+_ACT = {"IB_ACT": 1}              # the libraries whose kernels put an activation between bias and residual
+
+
+@functools.lru_cache(maxsize=4096)
+def _act_plan(M: int, N: int, K: int, sm_count: int):
+    """(swap, bn, splits) of a product with an activation, or None. As ``gemm_choice``, but slices of K meet in a cluster's shared memory
+    everywhere: a call then needs no scratch, and calls may run on any streams at once."""
+    plan = gemm_choice(M, N, K, sm_count)
+    if plan is None:
+        return None
+    swap, bn, splits, ws_floats, _ = plan
+    if ws_floats > 0:
+        kb = -(-K // 64)
+        splits = next((c for c in (8, 4, 2) if kb // c >= 2 and -(-kb // -(-kb // c)) == c), 1)
+    return swap, bn, splits
+
+
+def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], act: int, residual: Optional[torch.Tensor],
+               out: torch.Tensor) -> bool:
+    """``ops.linear_act`` (which has looked at the operands) as one kernel; False where none takes the operands."""
+    (M, K), N = x.shape, w.shape[0]
+    st = device_state(x.device)
+    px, pw, po = x.data_ptr(), w.data_ptr(), out.data_ptr()
+    pb, pr = _ptr(bias), _ptr(residual)
+    if x.dtype is torch.float32:
+        if out.dtype is not torch.float32:
+            return False
+        if _f32_act_on_tensor_cores(N, K):
+            f = _fn("lin32_tc", "ib_linear_f32_tc", _F32_TC_ACT_ARGS, _ACT)
+            _call(f, px, pw, pb, pr, po, M, N, K, st.sm_count, 1, act, st.status.data_ptr(), _stream())
+        else:
+            f = _fn("lin32", "ib_linear_f32", _F32_ACT_ARGS, _ACT)
+            _call(f, px, pw, pb, pr, po, M, N, K, 0, st.sm_count, 1, act, _stream())
+        return True
+    if K % 8 or (px & 15) or (pw & 15):
+        return False
+    if M <= skinny_limits()[0]:
+        f = _fn("gemvb", "ib_linear_skinny_act", _SKINNY_ACT_ARGS)
+        _call(f, px, pw, pb, pr, po, M, N, K, dtype_code(out.dtype), act, st.sm_count, st.status.data_ptr(), _stream())
+        return True
+    plan = _act_plan(M, N, K, st.sm_count)
+    if plan is None:
+        return False
+    f = _fn("gemm", "ib_gemm_tc", _GEMM_ACT_ARGS, _ACT)
+    _call(f, px, pw, pb, pr, po, M, N, K, dtype_code(out.dtype), act, *plan, None, None, st.status.data_ptr(), _stream())
+    return True
+
+
+_F32_TC_ACT_ARGS = [c_void_p] * 5 + [c_int64] * 3 + [c_int] * 3 + [c_void_p] * 2
+_F32_ACT_ARGS = [c_void_p] * 5 + [c_int64] * 3 + [c_int] * 4 + [c_void_p]
+_SKINNY_ACT_ARGS = [c_void_p] * 5 + [c_int64] * 3 + [c_int] * 3 + [c_void_p] * 2
+_GEMM_ACT_ARGS = [c_void_p] * 5 + [c_int64] * 3 + [c_int] * 5 + [c_void_p] * 4
+
+
+def _f32_act_on_tensor_cores(N: int, K: int) -> bool:
+    return N >= 128 and K >= 128
+
+
 def head_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[torch.Tensor], top: int, scale: float, softcap: float,
                   status: Optional[torch.Tensor]):
     """``ops.head_logprobs`` (which has looked at the operands) without logits in memory; None for rows that the streaming product takes

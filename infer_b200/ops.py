@@ -446,7 +446,8 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
     (0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3)))), "gelu" (0.5 z (1 + erf(z / sqrt 2))), "silu" (z / (1 + e^-z)). The result is
     float32 or bfloat16 (default: as x; with a residual float32). ``w`` is a loaded weight (as for ``linear``). A kernel whose bounded wait
     runs out says so in the device's status word."""
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise KernelError(f"activation {activation!r} is not among {sorted(ACTIVATIONS)}")
     _check_product("linear_act", x, w)
     (M, K), N, device = x.shape, w.shape[0], x.device
@@ -470,12 +471,16 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
     if M == 0:
         return out
     from . import fast_ops
-    z = fast_ops.linear(x, w, bias, None, torch.float32, None)
-    if z is None:
-        z = linear_plain(x, w, bias, None, torch.float32, w_ready=True)
-    f = _fn("score", "ib_act_residual", [c_void_p] * 3 + [c_int64, c_int, c_int, c_void_p])
-    _call(f, z.data_ptr(), _ptr(residual), out.data_ptr(), M * N, ACTIVATIONS[activation], dtype_code(out_dtype), _stream())
+    if fast_ops.linear_act(x, w, bias, act, residual, out):
+        return out
+    # rows that do not keep to 16 bytes, float32 rows into a bfloat16 result: the float sums first, then what is left to do
+    z = linear_plain(x, w, bias, None, torch.float32, w_ready=True)
+    f = _fn("score", "ib_act_residual", _ACT_RESIDUAL_ARGS)
+    _call(f, z.data_ptr(), _ptr(residual), out.data_ptr(), M * N, act, dtype_code(out_dtype), _stream())
     return out
+
+
+_ACT_RESIDUAL_ARGS = [c_void_p] * 3 + [c_int64, c_int, c_int, c_void_p]
 
 
 # ----------------------------------------------------------------------------- kernels of layers with state
