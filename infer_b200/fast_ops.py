@@ -324,44 +324,45 @@ def _act_plan(M: int, N: int, K: int, sm_count: int):
 
 
 def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], act: int, residual: Optional[torch.Tensor],
-               out: torch.Tensor) -> bool:
-    """``ops.linear_act`` (which has looked at the operands) as one kernel; False where none takes the operands."""
+               out: torch.Tensor, code: int) -> bool:
+    """``ops.linear_act`` (which has looked at the operands; ``code``: of the result's type) as one kernel; False where none takes them."""
     (M, K), N = x.shape, w.shape[0]
     st = device_state(x.device)
-    px, pw, po = x.data_ptr(), w.data_ptr(), out.data_ptr()
-    pb, pr = _ptr(bias), _ptr(residual)
+    px, pw = x.data_ptr(), w.data_ptr()
+    same = (px, pw, None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(), out.data_ptr(), M, N, K)
     if x.dtype is torch.float32:
-        if out.dtype is not torch.float32:
+        if code != 0:
             return False
-        if _f32_act_on_tensor_cores(N, K):
-            f = _fn("lin32_tc", "ib_linear_f32_tc", _F32_TC_ACT_ARGS, _ACT)
-            _call(f, px, pw, pb, pr, po, M, N, K, st.sm_count, 1, act, st.status.data_ptr(), _stream())
+        if _f32_act_on_tensor_cores(M, N, K):
+            _call(_act_fn("lin32_tc"), *same, st.sm_count, 1, act, st.status.data_ptr(), _stream())
         else:
-            f = _fn("lin32", "ib_linear_f32", _F32_ACT_ARGS, _ACT)
-            _call(f, px, pw, pb, pr, po, M, N, K, 0, st.sm_count, 1, act, _stream())
+            _call(_act_fn("lin32"), *same, 0, st.sm_count, 1, act, _stream())
         return True
     if K % 8 or (px & 15) or (pw & 15):
         return False
-    if M <= skinny_limits()[0]:
-        f = _fn("gemvb", "ib_linear_skinny_act", _SKINNY_ACT_ARGS)
-        _call(f, px, pw, pb, pr, po, M, N, K, dtype_code(out.dtype), act, st.sm_count, st.status.data_ptr(), _stream())
+    if M <= 16:
+        _call(_act_fn("gemvb"), *same, code, act, st.sm_count, st.status.data_ptr(), _stream())
         return True
     plan = _act_plan(M, N, K, st.sm_count)
     if plan is None:
         return False
-    f = _fn("gemm", "ib_gemm_tc", _GEMM_ACT_ARGS, _ACT)
-    _call(f, px, pw, pb, pr, po, M, N, K, dtype_code(out.dtype), act, *plan, None, None, st.status.data_ptr(), _stream())
+    _call(_act_fn("gemm"), *same, code, act, *plan, None, None, st.status.data_ptr(), _stream())
     return True
 
 
-_F32_TC_ACT_ARGS = [c_void_p] * 5 + [c_int64] * 3 + [c_int] * 3 + [c_void_p] * 2
-_F32_ACT_ARGS = [c_void_p] * 5 + [c_int64] * 3 + [c_int] * 4 + [c_void_p]
-_SKINNY_ACT_ARGS = [c_void_p] * 5 + [c_int64] * 3 + [c_int] * 3 + [c_void_p] * 2
-_GEMM_ACT_ARGS = [c_void_p] * 5 + [c_int64] * 3 + [c_int] * 5 + [c_void_p] * 4
+@functools.lru_cache(maxsize=None)
+def _act_fn(module: str):
+    name, args = {"lin32_tc": ("ib_linear_f32_tc", [c_int] * 3 + [c_void_p] * 2), "lin32": ("ib_linear_f32", [c_int] * 4 + [c_void_p]),
+                  "gemvb": ("ib_linear_skinny_act", [c_int] * 3 + [c_void_p] * 2), "gemm": ("ib_gemm_tc", [c_int] * 5 + [c_void_p] * 4)}[module]
+    return _fn(module, name, [c_void_p] * 5 + [c_int64] * 3 + args, None if module == "gemvb" else _ACT)
 
 
-def _f32_act_on_tensor_cores(N: int, K: int) -> bool:
-    return N >= 128 and K >= 128
+def _f32_act_on_tensor_cores(M: int, N: int, K: int) -> bool:
+    """Which of the 32-bit kernels, multiply-adds or the tensor cores with each float as three bfloat16 numbers, takes less time: measured (multiply-adds,
+    tensor cores; us) 1 x 2301 x 1000 4.2 and 8.9, 8 x 2301 x 1000 6.9 and 9.1, 64 x 1000 x 500 10.5 and 9.1, 301 x 300 x 300 8.4 and 17.2,
+    301 x 1000 x 200 11.1 and 15.9, 1000 x 500 x 500 25.5 and 14.6, 2000 x 1000 x 128 29.8 and 24.6, 8 x 16000 x 400 17.3 and 11.4,
+    333 x 32003 x 1000 643 and 294. (Not by N and K alone as the engine's products: a row's bits may depend on how many rows there are.)"""
+    return N >= 128 and K >= 128 and M >= 2 and M * N * K >= 30_000_000
 
 
 def head_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[torch.Tensor], top: int, scale: float, softcap: float,
@@ -372,17 +373,28 @@ def head_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[torch.Tenso
     T, H = x.shape
     if T <= skinny_limits()[0] or H % 8 or (x.data_ptr() & 15) or (w.data_ptr() & 15):
         return None
-    sms, nbytes = ops.sm_count(x.device), c_int64()
-    f = _fn("score_head", "ib_head_logprobs_scratch", [c_int64] * 3 + [c_int] * 2 + [c_void_p])
-    if f(T, w.shape[0], H, top, sms, ctypes.byref(nbytes)) != 0:
+    sms = ops.sm_count(x.device)
+    nbytes = _head_scratch(T, w.shape[0], H, top, sms)
+    if nbytes is None:
         return None
-    r = ops._new_logprobs(T, top, x)
-    scratch = x.new_empty((nbytes.value,), dtype=torch.uint8)
-    f = _fn("score_head", "ib_head_logprobs", [c_void_p] * 2 + [c_int64] * 3 + [c_void_p, c_int, c_float, c_float] + [c_void_p] * 5 + [c_int] + [c_void_p] * 2)
-    _call(f, x.data_ptr(), w.data_ptr(), T, w.shape[0], H, _ptr(tokens), top, float(scale), float(softcap), r.logprob.data_ptr(),
+    r = ops._new_logprobs(T, top, x.device)
+    scratch = x.new_empty((nbytes,), dtype=torch.uint8)
+    _call(_head_fn(), x.data_ptr(), w.data_ptr(), T, w.shape[0], H, _ptr(tokens), top, float(scale), float(softcap), r.logprob.data_ptr(),
           r.entropy.data_ptr(), r.top_ids.data_ptr(), r.top_logprobs.data_ptr(), scratch.data_ptr(), sms,
           (device_state(x.device).status if status is None else status).data_ptr(), _stream())
     return r
+
+
+@functools.lru_cache(maxsize=4096)
+def _head_scratch(T: int, V: int, H: int, top: int, sm_count: int) -> Optional[int]:
+    nbytes = c_int64()
+    f = _fn("score_head", "ib_head_logprobs_scratch", [c_int64] * 3 + [c_int] * 2 + [c_void_p])
+    return nbytes.value if f(T, V, H, top, sm_count, ctypes.byref(nbytes)) == 0 else None
+
+
+@functools.lru_cache(maxsize=None)
+def _head_fn():
+    return _fn("score_head", "ib_head_logprobs", [c_void_p] * 2 + [c_int64] * 3 + [c_void_p, c_int, c_float, c_float] + [c_void_p] * 5 + [c_int] + [c_void_p] * 2)
 
 
 GROUPED_FROM = 256            # tokens from which a routed feed-forward's rows are worth grouping by expert

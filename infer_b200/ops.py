@@ -312,12 +312,6 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: torch.Tensor
 
 
-@functools.lru_cache(maxsize=None)
-def max_top_logprobs() -> int:
-    """The most alternatives that a call may ask for."""
-    return int(_fn("score", "ib_max_top_logprobs", [])())
-
-
 def _check_logprobs(rows: int, device, tokens: Optional[torch.Tensor], status: Optional[torch.Tensor]) -> None:
     for name, t, n in (("tokens", tokens, rows), ("status", status, 1)):
         if t is None:
@@ -328,20 +322,25 @@ def _check_logprobs(rows: int, device, tokens: Optional[torch.Tensor], status: O
             raise KernelError(f"{name} must lie on {device}, not on {t.device}")
 
 
-def _check_distribution(top: int, scale: float, softcap: float) -> None:
-    if not 0 <= top <= max_top_logprobs():
-        raise KernelError(f"0 to {max_top_logprobs()} alternatives can be asked for, not {top}")
-    if not (0 < scale < math.inf):
+def _refuse_distribution(top: int, scale: float, softcap: float) -> None:
+    if not 0 <= top <= 20:
+        raise KernelError(f"0 to 20 alternatives can be asked for, not {top}")
+    if not 0 < scale < math.inf:
         raise KernelError(f"the logits' scale must be positive and finite, not {scale}")
-    if not (0 <= softcap < math.inf):
-        raise KernelError(f"the logits' cap must be positive and finite, or 0 for none, not {softcap}")
+    raise KernelError(f"the logits' cap must be positive and finite, or 0 for none, not {softcap}")
 
 
-def _new_logprobs(rows: int, top: int, like: torch.Tensor) -> TokenLogprobs:
-    """Results on the device of ``like``. (new_empty: half a microsecond less than empty, four times a call.)"""
-    f32 = torch.float32
-    return TokenLogprobs(like.new_empty((rows,), dtype=f32), like.new_empty((rows,), dtype=f32),
-                         like.new_empty((rows, top), dtype=torch.int32), like.new_empty((rows, top), dtype=f32))
+@functools.lru_cache(maxsize=64)
+def _logprobs_like(rows: int, top: int, device: torch.device):
+    one, ids = torch.empty(1, dtype=torch.float32, device=device), torch.empty(1, dtype=torch.int32, device=device)
+    return one.expand(rows), ids.expand(rows, top), one.expand(rows, top)
+
+
+def _new_logprobs(rows: int, top: int, device: torch.device) -> TokenLogprobs:
+    """(empty_like a kept tensor of the size, of one element expanded: 1.3 us a tensor where empty takes 2.3, four times a call.)"""
+    a, ids, b = _logprobs_like(rows, top, device)
+    new, flat = torch.empty_like, torch.contiguous_format
+    return TokenLogprobs(new(a, memory_format=flat), new(a, memory_format=flat), new(ids, memory_format=flat), new(b, memory_format=flat))
 
 
 def _logprobs_cluster(rows: int, vocab: int, sm_count: int) -> int:
@@ -365,26 +364,29 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     [0, V): NaN, and the status word (if given) is set to 1. ``scale`` / ``softcap``: the distribution is that of
     softcap * tanh(logits * scale / softcap) (-inf stays -inf), or logits * scale without a cap; alternatives go by ``logits``.
     Each call may run on any stream; a captured one reads its inputs anew at each replay."""
-    _check_distribution(top, scale, softcap)
-    _check(logits, "logits", torch.float32)
-    if logits.dim() != 2 or logits.shape[1] < 1:
-        raise KernelError(f"logits must be [rows, vocabulary], got {tuple(logits.shape)}")
-    T, V = logits.shape
-    device = logits.device
+    if not (0 <= top <= 20 and 0 < scale < math.inf and 0 <= softcap < math.inf):
+        _refuse_distribution(top, scale, softcap)
+    if not logits.is_cuda or logits.dtype is not torch.float32 or not logits.is_contiguous():
+        _check(logits, "logits", torch.float32)
+    shape, device = logits.shape, logits.device
+    if len(shape) != 2 or shape[1] < 1:
+        raise KernelError(f"logits must be [rows, vocabulary], got {tuple(shape)}")
+    T, V = shape
     if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return token_logprobs(logits, tokens, top, status, scale, softcap, out)
     _check_logprobs(T, device, tokens, status)
-    r = _new_logprobs(T, top, logits) if out is None else out
+    r = _new_logprobs(T, top, device) if out is None else out
     if T == 0:
         return r
-    f = _fn("score", "ib_token_logprobs", _TOKEN_LOGPROBS_ARGS)
-    _call(f, logits.data_ptr(), T, V, _ptr(tokens), top, scale, softcap, r.logprob.data_ptr(), r.entropy.data_ptr(),
+    _call(_token_logprobs_fn(), logits.data_ptr(), T, V, _ptr(tokens), top, scale, softcap, r.logprob.data_ptr(), r.entropy.data_ptr(),
           r.top_ids.data_ptr(), r.top_logprobs.data_ptr(), _logprobs_cluster(T, V, sm_count(device)), _ptr(status), _stream())
     return r
 
 
-_TOKEN_LOGPROBS_ARGS = [c_void_p, c_int64, c_int64, c_void_p, c_int, c_float, c_float] + [c_void_p] * 4 + [c_int] + [c_void_p] * 2
+@functools.lru_cache(maxsize=None)
+def _token_logprobs_fn():
+    return _fn("score", "ib_token_logprobs", [c_void_p, c_int64, c_int64, c_void_p, c_int, c_float, c_float] + [c_void_p] * 4 + [c_int] + [c_void_p] * 2)
 
 
 @functools.lru_cache(maxsize=None)
@@ -398,37 +400,40 @@ def head_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[torch.Tenso
     not kept: bfloat16 rows go through a kernel that holds them in tensor memory only; up to 16 rows, rows that do not keep to 16 bytes and
     float32 go through logits of a few rows at a time. ``w`` is a loaded weight (as for ``linear``). A kernel whose bounded wait runs out
     says so in the device's status word."""
-    _check_distribution(top, scale, softcap)
+    if not (0 <= top <= 20 and 0 < scale < math.inf and 0 <= softcap < math.inf):
+        _refuse_distribution(top, scale, softcap)
     _check_product("head_logprobs", x, w)
     (T, K), V, device = x.shape, w.shape[0], x.device
     if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return head_logprobs(x, w, tokens, top, scale, softcap, status)
     _check_logprobs(T, device, tokens, status)
-    from . import fast_ops
     if T > 0 and x.dtype is torch.bfloat16:
+        from . import fast_ops
         r = fast_ops.head_logprobs(x, w, tokens, top, scale, softcap, status)
         if r is not None:
             return r
-    r = _new_logprobs(T, top, x)
+    r = _new_logprobs(T, top, device)
     step = max(1, min(T, HEAD_LOGITS // V))
     logits = x.new_empty((step, V), dtype=torch.float32)
     for lo in range(0, T, step):
         hi = min(T, lo + step)
         z, rows, part, here = (logits, x, r, tokens) if step == T else \
             (logits[:hi - lo], x[lo:hi], TokenLogprobs(*(t[lo:hi] for t in r)), None if tokens is None else tokens[lo:hi])
-        if fast_ops.linear(rows, w, None, None, torch.float32, z) is None:
-            linear_plain(rows, w, out=z, w_ready=True)
+        linear_act(rows, w, out=z)
         token_logprobs(z, here, top, status, scale, softcap, part)
     return r
 
 
 def _check_product(what: str, x: torch.Tensor, w: torch.Tensor) -> None:
-    _check(x, "x")
-    _check(w, "w", x.dtype)
-    dtype_code(x.dtype)
-    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or 0 in w.shape:
-        raise KernelError(f"{what}: x is {tuple(x.shape)} but w is {tuple(w.shape)}")
+    dtype = x.dtype
+    if not (x.is_cuda and w.is_cuda and w.dtype is dtype and x.is_contiguous() and w.is_contiguous() and dtype in _DTYPE_CODE):
+        _check(x, "x")
+        dtype_code(dtype)
+        _check(w, "w", dtype)
+    a, b = x.shape, w.shape
+    if len(a) != 2 or len(b) != 2 or a[1] != b[1] or b[0] < 1 or b[1] < 1:
+        raise KernelError(f"{what}: x is {tuple(a)} but w is {tuple(b)}")
     if w.device != x.device:
         raise KernelError(f"w must lie on {x.device}, not on {w.device}")
 
@@ -451,18 +456,14 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
         raise KernelError(f"activation {activation!r} is not among {sorted(ACTIVATIONS)}")
     _check_product("linear_act", x, w)
     (M, K), N, device = x.shape, w.shape[0], x.device
-    if bias is not None:
-        _check(bias, "bias", torch.float32, (N,))
-    if residual is not None:
-        _check(residual, "residual", torch.float32, (M, N))
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else torch.float32 if residual is not None else x.dtype
-    dtype_code(out_dtype)
-    if out is not None:
-        _check(out, "out", out_dtype, (M, N))
-    for name, t in (("bias", bias), ("residual", residual), ("out", out)):
-        if t is not None and t.device != device:
-            raise KernelError(f"{name} must lie on {device}, not on {t.device}")
+    code = dtype_code(out_dtype)
+    for name, t, dtype, shape in (("bias", bias, torch.float32, (N,)), ("residual", residual, torch.float32, (M, N)), ("out", out, out_dtype, (M, N))):
+        if t is not None:
+            _check(t, name, dtype, shape)
+            if t.device != device:
+                raise KernelError(f"{name} must lie on {device}, not on {t.device}")
     if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return linear_act(x, w, bias, activation, residual, out_dtype, out)
@@ -471,12 +472,12 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
     if M == 0:
         return out
     from . import fast_ops
-    if fast_ops.linear_act(x, w, bias, act, residual, out):
+    if fast_ops.linear_act(x, w, bias, act, residual, out, code):
         return out
     # rows that do not keep to 16 bytes, float32 rows into a bfloat16 result: the float sums first, then what is left to do
     z = linear_plain(x, w, bias, None, torch.float32, w_ready=True)
     f = _fn("score", "ib_act_residual", _ACT_RESIDUAL_ARGS)
-    _call(f, z.data_ptr(), _ptr(residual), out.data_ptr(), M * N, act, dtype_code(out_dtype), _stream())
+    _call(f, z.data_ptr(), _ptr(residual), out.data_ptr(), M * N, act, code, _stream())
     return out
 
 
