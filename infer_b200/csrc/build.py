@@ -44,6 +44,7 @@ MODULES: Dict[str, str] = {
     "latent_pf": "latent_prefill.cu",   # the same attention for prompt portions: per-head keys and values, tensor cores
     "score": "score_ops.cu",     # log probabilities, entropies and alternatives from logits; activations behind a product
     "score_head": "score_head.cu",      # the same from the rows in front of a head, the logits in tensor memory only
+    "act_tc": "act_tcgen05.cu",  # products with an activation between bias and residual, on pairs of SMs
     "gemvb": "gemv_bulk.cu",
     "gemm": "gemm_tcgen05.cu",
     "attn": "attention_fast.cu",

@@ -45,8 +45,8 @@
 #include <mutex>
 #include <unordered_map>
 
-// Compiled with IB_ACT the same kernels put an activation between bias and residual (a library of its own: the products without one stay
-// as they are).
+// Compiled with IB_ACT the kernels of the swapped mapping put an activation between bias and residual (a library of its own, for up to 128 rows: the
+// products without one stay as they are; act_tcgen05.cu takes more rows).
 #ifdef IB_ACT
 #include "score.cuh"
 #define IB_ACTIVATE_ALL(p, x) ib::score::activate_all<16>(x, (p).act)
@@ -1356,6 +1356,7 @@ IB_EXPORT int ib_gemm_tc(const void* x, const void* w, const float* bias, const 
 #ifdef IB_ACT
     const int act = epi;                                          // (the library with activations has no other epilogues)
     if (act < 0 || act >= ib::score::ACTIVATIONS) return ib::fail(IB_ERR_ARG, "gemm_tc: unknown activation %d", act);
+    if (!swap || bn > 128) return ib::fail(IB_ERR_ARG, "gemm_tc: activations come with the swapped mapping");
     epi = 0;
 #endif
     if (epi != 0 && epi != 2) return ib::fail(IB_ERR_ARG, "gemm_tc: unknown epilogue %d", epi);
@@ -1389,6 +1390,7 @@ IB_EXPORT int ib_gemm_tc(const void* x, const void* w, const float* bias, const 
     const bool f32 = out_dtype == IB_F32;
     if (!f32 && out_dtype != IB_BF16) return ib::fail(IB_ERR_ARG, "gemm_tc: unknown output dtype %d", out_dtype);
     CUtensorMap ma, mb;
+#ifndef IB_ACT
     if (bn >= 256 && !sliced_wide) {
         const bool wide = bn >= 352 && bn <= 512, paired = bn >= 1280;
         const int width = paired ? (bn - 1024) / 2 : wide ? bn / 2 : 128;
@@ -1419,14 +1421,17 @@ IB_EXPORT int ib_gemm_tc(const void* x, const void* w, const float* bias, const 
         if (bn == 352) return f32 ? launch_persistent<176, true, float>(ma, mb, p, sms, stream) : launch_persistent<176, true, bf16>(ma, mb, p, sms, stream);
         return f32 ? launch_persistent<128, false, float>(ma, mb, p, sms, stream) : launch_persistent<128, false, bf16>(ma, mb, p, sms, stream);
     }
+#endif
     int rc = get_map(swap ? w : x, p.rows_a, K, BM, &ma);
     if (rc) return rc;
     rc = get_map(swap ? x : w, p.rows_b, K, bn, &mb);
     if (rc) return rc;
+#ifndef IB_ACT
     if (sliced_wide) {
         p.stages = p.kb_per_split >= 4 ? 4 : 3;          // the ring also receives the slices' columns: 128 KB
         return f32 ? launch<256, float>(ma, mb, p, grid, stream) : launch<256, bf16>(ma, mb, p, grid, stream);
     }
+#endif
     p.stages = bn == 16 ? pick_stages<16>(p) : bn == 32 ? pick_stages<32>(p) : bn == 64 ? pick_stages<64>(p) : pick_stages<128>(p);
     switch (bn) {
         case 16: return f32 ? launch<16, float>(ma, mb, p, grid, stream) : launch<16, bf16>(ma, mb, p, grid, stream);

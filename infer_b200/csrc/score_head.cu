@@ -171,6 +171,8 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     auto empty_bar = [&](int s) { return bars + 8u * (S + s); };
     auto acc_full_bar = [&](int b) { return bars + 8u * (2 * S + b); };
     auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * S + 2 + b); };
+    // CTAs of different chunks go through K from different places on, or all SMs would ask the same few L2 slices for x at a time
+    auto first_kb = [&](int chunk) { return int(int64_t(chunk) * ((n_kb + KPS - 1) / KPS) / p.chunks) * KPS; };
     auto first_tile = [&](int chunk) { return int(int64_t(chunk) * p.tiles_n / p.chunks); };
 
     if (threadIdx.x == 0) {
@@ -209,7 +211,7 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                 const int t_end = first_tile(chunk + 1);
                 for (int tile = first_tile(chunk); tile < t_end && !slots[1]; tile++) {
                     const int b_row = tile * p.width + int(rank) * b_rows;
-                    for (int kb = 0; kb < n_kb; kb += KPS, it++) {
+                    for (int i = 0, kb = first_kb(chunk); i < n_kb; i += KPS, kb = kb + KPS < n_kb ? kb + KPS : 0, it++) {
                         const int n = min(KPS, n_kb - kb);
                         if (it >= S && !mbar_wait(empty_bar(s), parity)) {
                             atomicExch(p.status, STATUS_TIMEOUT_PRODUCER); slots[1] = 1; break;
@@ -249,21 +251,21 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                     if (lt >= 2 && !mbar_wait_each(acc_empty_bar(b), ((lt >> 1) - 1) & 1)) { ok = false; break; }      // it has been drained
                     tc_fence_after();
                     const uint32_t d = tmem_base + uint32_t(b * 256);
-                    for (int kb = 0; kb < n_kb; kb += KPS) {
+                    for (int k0 = 0, kb = first_kb(chunk); k0 < n_kb; k0 += KPS, kb = kb + KPS < n_kb ? kb + KPS : 0) {
                         if (!mbar_wait_each(full_bar(s), parity)) { ok = false; break; }
                         const uint32_t a_addr = base + s * R::STAGE_BYTES;
                         const uint64_t ad = make_desc(a_addr, 16, 1024), bd = make_desc(a_addr + KPS * A_BYTES, 16, 1024);
                         if (leader) {
 #pragma unroll
                             for (int k = 0; k < BK / UMMA_K; k++)
-                                umma<CG>(d, ad + uint64_t(2 * k), bd + uint64_t(2 * k), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                                umma<CG>(d, ad + uint64_t(2 * k), bd + uint64_t(2 * k), idesc, (k0 > 0 || k > 0) ? 1u : 0u);
                             if (KPS == 2 && kb + 1 < n_kb) {
 #pragma unroll
                                 for (int k = 0; k < BK / UMMA_K; k++)
                                     umma<CG>(d, ad + uint64_t((A_BYTES >> 4) + 2 * k), bd + uint64_t((R::B_BYTES >> 4) + 2 * k), idesc, 1u);
                             }
                             commit<CG>(empty_bar(s));
-                            if (kb + KPS >= n_kb) commit<CG>(acc_full_bar(b));
+                            if (k0 + KPS >= n_kb) commit<CG>(acc_full_bar(b));
                         }
                         __syncwarp();
                         if (++s == S) { s = 0; parity ^= 1u; }

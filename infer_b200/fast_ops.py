@@ -311,16 +311,15 @@ _ACT = {"IB_ACT": 1}              # the libraries whose kernels put an activatio
 
 @functools.lru_cache(maxsize=4096)
 def _act_plan(M: int, N: int, K: int, sm_count: int):
-    """(swap, bn, splits) of a product with an activation, or None. As ``gemm_choice``, but slices of K meet in a cluster's shared memory
-    everywhere: a call then needs no scratch, and calls may run on any streams at once."""
-    plan = gemm_choice(M, N, K, sm_count)
-    if plan is None:
-        return None
-    swap, bn, splits, ws_floats, _ = plan
-    if ws_floats > 0:
-        kb = -(-K // 64)
-        splits = next((c for c in (8, 4, 2) if kb // c >= 2 and -(-kb // -(-kb // c)) == c), 1)
-    return swap, bn, splits
+    """What a product with an activation runs as: (True, tile width, slices of K) on pairs of SMs, (False, columns of a tile, slices of K) for
+    up to 128 rows, whose slices meet in a cluster's shared memory (neither needs scratch: calls may run on any streams at once);
+    None if the sizes are refused."""
+    if M <= 128:
+        plan = gemm_plan(M, N, K, sm_count)
+        return None if plan is None else (False, plan[1], plan[2])
+    width, slices = c_int(), c_int()
+    f = _fn("act_tc", "ib_linear_act_plan", [c_int64] * 3 + [c_int] + [c_void_p] * 2)
+    return (True, width.value, slices.value) if f(M, N, K, sm_count, ctypes.byref(width), ctypes.byref(slices)) == 0 else None
 
 
 def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], act: int, residual: Optional[torch.Tensor],
@@ -346,15 +345,20 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], a
     plan = _act_plan(M, N, K, st.sm_count)
     if plan is None:
         return False
-    _call(_act_fn("gemm"), *same, code, act, *plan, None, None, st.status.data_ptr(), _stream())
+    pairs, width, slices = plan
+    if pairs:
+        _call(_act_fn("act_tc"), *same, code, act, width, slices, st.sm_count, st.status.data_ptr(), _stream())
+    else:
+        _call(_act_fn("gemm"), *same, code, act, 1, width, slices, None, None, st.status.data_ptr(), _stream())
     return True
 
 
 @functools.lru_cache(maxsize=None)
 def _act_fn(module: str):
     name, args = {"lin32_tc": ("ib_linear_f32_tc", [c_int] * 3 + [c_void_p] * 2), "lin32": ("ib_linear_f32", [c_int] * 4 + [c_void_p]),
-                  "gemvb": ("ib_linear_skinny_act", [c_int] * 3 + [c_void_p] * 2), "gemm": ("ib_gemm_tc", [c_int] * 5 + [c_void_p] * 4)}[module]
-    return _fn(module, name, [c_void_p] * 5 + [c_int64] * 3 + args, None if module == "gemvb" else _ACT)
+                  "gemvb": ("ib_linear_skinny_act", [c_int] * 3 + [c_void_p] * 2), "gemm": ("ib_gemm_tc", [c_int] * 5 + [c_void_p] * 4),
+                  "act_tc": ("ib_linear_act", [c_int] * 5 + [c_void_p] * 2)}[module]
+    return _fn(module, name, [c_void_p] * 5 + [c_int64] * 3 + args, None if module in ("gemvb", "act_tc") else _ACT)
 
 
 def _f32_act_on_tensor_cores(M: int, N: int, K: int) -> bool:

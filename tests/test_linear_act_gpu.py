@@ -74,6 +74,49 @@ def test_bfloat16(M, N, K):
     assert st.status.item() == 0
 
 
+# tile width, slices of K: every kernel on pairs of SMs, with ragged rows and columns, K of one k-block to several chains, odd numbers of k-blocks
+@pytest.mark.parametrize("width,slices", [(32, 1), (64, 1), (96, 2), (128, 4), (160, 1), (192, 4), (224, 4), (256, 1), (256, 2), (32, 4)])
+@pytest.mark.parametrize("M,N,K", [(129, 40, 72), (300, 301, 520), (257, 520, 1160), (600, 1000, 2056), (1, 9, 1024)])
+def test_pairs_of_sms(width, slices, M, N, K):
+    from infer_b200 import fast_ops, ops
+    if slices > 1 and -(-K // 64) < 2 * slices:
+        slices = 1
+    x, w, bias, res = _operands(M, N, K, torch.bfloat16)
+    st = fast_ops.device_state(DEV)
+    st.status.zero_()
+    for dtype, code in ((torch.float32, 0), (torch.bfloat16, 1)):
+        for act, b, r in ((0, None, None), (3, bias, None), (5, bias, res), (2, None, res)):
+            out = torch.full((M, N), 7.0, dtype=dtype, device=DEV)
+            ops._call(fast_ops._act_fn("act_tc"), x.data_ptr(), w.data_ptr(), None if b is None else b.data_ptr(), None if r is None else r.data_ptr(),
+                      out.data_ptr(), M, N, K, code, act, width, slices, st.sm_count, st.status.data_ptr(), ops._stream())
+            check(out, x, w, b, ACTS[act], r)
+    assert st.status.item() == 0
+
+
+@pytest.mark.parametrize("M,N,K", [(600, 512, 18944), (140, 256, 8960), (2048, 128, 8960)])
+def test_long_sums_keep_their_digits(M, N, K):
+    """Float results: chains of 512 elements, each off by at most 2^-23 of its running sum at each of 32 steps, below 32 x 2^-23 / 2 of its size on average
+    and 1e-6 of the whole in norm (the chains' errors add up as their sizes do); one chain over K would be 1e-5 off."""
+    from infer_b200 import ops
+    x, w, bias, res = _operands(M, N, K, torch.bfloat16)
+    y = ops.linear_act(x, w, None, "none", None, torch.float32).double()
+    z = x.double() @ w.double().t()
+    assert ((y - z).norm() / z.norm()).item() < 2e-6
+
+
+@pytest.mark.parametrize("M", [8, 60, 200])
+def test_results_and_residuals_that_start_anywhere(M):
+    from infer_b200 import ops
+    N = 64
+    x, w, bias, res = _operands(M, N, 256, torch.bfloat16)
+    for shift in (1, 2, 3):
+        r = torch.empty(M * N + shift, device=DEV)[shift:].view(M, N).copy_(res)
+        for dtype in (torch.float32, torch.bfloat16):
+            out = torch.empty(M * N + shift, dtype=dtype, device=DEV)[shift:].view(M, N)
+            b = torch.empty(N + shift, device=DEV)[shift:].copy_(bias)
+            check(ops.linear_act(x, w, b, "gelu", r, dtype, out), x, w, bias, "gelu", res)
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 1, 1), (3, 37, 65), (8, 300, 1000), (17, 1030, 1024), (301, 2301, 1000), (130, 1500, 2048), (64, 100, 7)])
 def test_float32(M, N, K):
     from infer_b200 import ops
