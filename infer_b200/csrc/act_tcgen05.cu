@@ -7,8 +7,8 @@
 // for a tile's gelu as the tile's MMAs at K = 1536).
 //
 // The tensor core's additions into an accumulator truncate, and the error of a long chain has one sign: 1e-5 of the result after 8,960 elements of
-// K. Where the result is float (SUMS), an accumulator starts anew every 512 elements and the warps add what it holds to sums in
-// registers: 128 a thread, which is why a thread has half of a row's columns. The additions run under the next 512 elements' MMAs.
+// K. Where the result is float (SUMS), an accumulator starts anew every 768 elements (below 1e-6) and the warps add what it holds to sums in
+// registers: 128 a thread, which is why a thread has half of a row's columns. The additions run under the next 768 elements' MMAs.
 //
 // A long K on few tiles is cut into S = 2 or 4 slices, the pairs of a cluster of 2 S CTAs. Each adds up its slice in registers; when all MMAs of
 // the cluster are done, every CTA pushes its columns to the CTAs that own them (a quarter or half each, of its own rows) through
@@ -31,11 +31,13 @@ using bf16 = __nv_bfloat16;
 constexpr int BM = 128, BK = 64, UMMA_K = 16, EPILOGUE_WARPS = 8, NUM_THREADS = 64 + 32 * EPILOGUE_WARPS;
 constexpr int STAGES = 3, MAX_WIDTH = 256, TMEM_COLS = 512;
 constexpr int A_BYTES = BM * BK * 2, B_BYTES = MAX_WIDTH / 2 * BK * 2, STAGE_BYTES = 2 * (A_BYTES + B_BYTES);
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
-constexpr int CHAIN = 8;                          // k-blocks that an accumulator adds up before the registers take over (SUMS)
+constexpr int BARS_BYTES = 256, BLOCK_BYTES = 32 * 16 * 4;        // BLOCK: a warp's 32 rows x 16 columns on their way to global memory
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + BARS_BYTES + EPILOGUE_WARPS * BLOCK_BYTES;
+constexpr int CHAIN = 12;                         // k-blocks that an accumulator adds up before the registers take over (SUMS)
 constexpr int COLS = MAX_WIDTH / 2;               // most columns of a thread
 constexpr int STATUS_TIMEOUT_PRODUCER = 151, STATUS_TIMEOUT_MMA = 152, STATUS_TIMEOUT_EPILOGUE = 153;
-static_assert(MAX_WIDTH * BM * 4 <= STAGES * STAGE_BYTES, "the slices' columns lie in the ring");
+constexpr int GROUP_BYTES = BM * 16 + 32;         // four columns of a CTA's rows, as slices send them
+static_assert(MAX_WIDTH / 4 * GROUP_BYTES <= STAGES * STAGE_BYTES, "the slices' columns lie in the ring");
 
 __device__ __forceinline__ void fence_barrier_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
@@ -86,69 +88,130 @@ __device__ __forceinline__ void tmem_get16(uint32_t taddr, float (&v)[16]) {
 struct ActParams {
     int64_t M, N;
     int n_kb, width, tiles_m, tiles_n, slices;
-    int act, vec;                // vec: rows of out and residual start on 16 bytes
+    int act, vec;                // vec: four columns of out (16 or 8 bytes) and residual (16) start on such a boundary
     const float* bias;           // [N] or null
     const float* residual;       // [M, N] or null (may be out)
     void* out;
     int* status;
 };
 
-// Finishes NC (a multiple of 4) neighbouring columns of one row.
-template <typename TOut, int NC>
-__device__ __forceinline__ void finish(const ActParams& p, int64_t m, int64_t n0, float (&v)[NC]) {
-    if (m >= p.M || n0 >= p.N) return;
-    TOut* out = static_cast<TOut*>(p.out) + m * p.N + n0;
-    const float* res = p.residual ? p.residual + m * p.N + n0 : nullptr;
-    const bool whole = p.vec && n0 + NC <= p.N;
-    float add[NC];
+// Four times four neighbouring columns that a lane finishes: number i starts `at` + i step elements into the result, with left - i less columns up to
+// the row's end, and is there if bit i of `live` is set.
+struct Four {
+    int64_t at, step;
+    int left, less;
+    uint32_t live;
+};
+__device__ __forceinline__ void residual_of(const ActParams& p, const Four& f, float4 (&add)[4]) {
 #pragma unroll
-    for (int j = 0; j < NC; j++) add[j] = 0.0f;
-    if (res) {                                                    // (all of it before the first store: it may be the output)
-        if (whole) {
+    for (int i = 0; i < 4; i++) {
+        add[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (!(f.live >> i & 1)) continue;
+        const float* at = p.residual + f.at + i * f.step;
+        if (p.vec) { add[i] = *reinterpret_cast<const float4*>(at); continue; }
+        const int left = f.left - i * f.less;
+        add[i].x = at[0];
+        if (left > 1) add[i].y = at[1];
+        if (left > 2) add[i].z = at[2];
+        if (left > 3) add[i].w = at[3];
+    }
+}
+__device__ __forceinline__ float4 bias_of(const ActParams& p, int64_t n) {
+    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (!p.bias) return f;
+    if (n < p.N) f.x = __ldg(p.bias + n);
+    if (n + 1 < p.N) f.y = __ldg(p.bias + n + 1);
+    if (n + 2 < p.N) f.z = __ldg(p.bias + n + 2);
+    if (n + 3 < p.N) f.w = __ldg(p.bias + n + 3);
+    return f;
+}
+// v[4 i + j] = column j of number i with its bias. ACT < 0: which activation is a parameter of the launch.
+template <int ACT, typename TOut>
+__device__ __forceinline__ void finish_four(const ActParams& p, const Four& f, float (&v)[16], const float4 (&add)[4]) {
+    if constexpr (ACT < 0) ib::score::activate_all<16>(v, p.act);
+    else {
 #pragma unroll
-            for (int j = 0; j < NC; j += 4) {
-                const float4 f = *reinterpret_cast<const float4*>(res + j);
-                add[j] = f.x; add[j + 1] = f.y; add[j + 2] = f.z; add[j + 3] = f.w;
+        for (int i = 0; i < 16; i++) v[i] = ib::score::activate(v[i], ACT);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (!(f.live >> i & 1)) continue;
+        const float x = v[4 * i] + add[i].x, y = v[4 * i + 1] + add[i].y, z = v[4 * i + 2] + add[i].z, w = v[4 * i + 3] + add[i].w;
+        TOut* at = static_cast<TOut*>(p.out) + f.at + i * f.step;
+        if (p.vec) {
+            if constexpr (sizeof(TOut) == 4) *reinterpret_cast<float4*>(at) = make_float4(x, y, z, w);
+            else {
+                const __nv_bfloat162 a = __floats2bfloat162_rn(x, y), b = __floats2bfloat162_rn(z, w);
+                *reinterpret_cast<uint2*>(at) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
             }
         } else {
-#pragma unroll
-            for (int j = 0; j < NC; j++) if (n0 + j < p.N) add[j] = res[j];
+            const int left = f.left - i * f.less;
+            at[0] = ib::from_f32<TOut>(x);
+            if (left > 1) at[1] = ib::from_f32<TOut>(y);
+            if (left > 2) at[2] = ib::from_f32<TOut>(z);
+            if (left > 3) at[3] = ib::from_f32<TOut>(w);
         }
-    }
-    if (p.bias) {
-#pragma unroll
-        for (int j = 0; j < NC; j++) v[j] += n0 + j < p.N ? __ldg(p.bias + n0 + j) : 0.0f;
-    }
-    ib::score::activate_all<NC>(v, p.act);
-#pragma unroll
-    for (int j = 0; j < NC; j++) v[j] += add[j];
-    if (whole) {
-        if constexpr (sizeof(TOut) == 4) {
-#pragma unroll
-            for (int j = 0; j < NC; j += 4) *reinterpret_cast<float4*>(out + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-        } else {
-            uint32_t h[NC / 2];
-#pragma unroll
-            for (int j = 0; j < NC / 2; j++) {
-                const __nv_bfloat162 two = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-                h[j] = *reinterpret_cast<const uint32_t*>(&two);
-            }
-            if constexpr (NC % 8 == 0) {
-#pragma unroll
-                for (int j = 0; j < NC / 2; j += 4) *reinterpret_cast<uint4*>(out + 2 * j) = make_uint4(h[j], h[j + 1], h[j + 2], h[j + 3]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < NC / 2; j += 2) *reinterpret_cast<uint2*>(out + 2 * j) = make_uint2(h[j], h[j + 1]);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < NC; j++) if (n0 + j < p.N) out[j] = ib::from_f32<TOut>(v[j]);
     }
 }
 
+// The columns of a warp's 32 rows of a finished tile, 16 at a time. They pass through the warp's block of shared memory, so that four lanes share
+// a row's 64 bytes: with a row a lane, a store of the warp touched 32 lines, and a tile of float results took longer to store than to
+// multiply at K = 1536. Units of 16 bytes, those of two rows in a line, are exchanged so that no two lanes meet in a bank. The bias is
+// read once a tile and the residual a block ahead: a trip to L2 for each block took 1,300 cycles of its 1,600.
+struct TileEnd {
+    Four f;                      // of the tile's first 16 columns
+    uint32_t rows;
+    float4 bias, add[4];         // bias: of columns 4 lane on
+    __device__ __forceinline__ void open(const ActParams& p, int64_t m0, int64_t n0) {
+        const int lane = threadIdx.x & 31, unit = lane & 3;
+        const int64_t m = m0 + (lane >> 2);
+        f.at = m * p.N + n0 + 4 * unit;
+        f.step = 8 * p.N;
+        f.left = int(p.N - n0) - 4 * unit;
+        f.less = 0;
+        rows = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) rows |= m + 8 * i < p.M ? 1u << i : 0u;
+        f.live = f.left > 0 ? rows : 0u;
+        bias = bias_of(p, n0 + 4 * lane);
+#pragma unroll
+        for (int i = 0; i < 4; i++) add[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (p.residual) residual_of(p, f, add);
+    }
+    // v: this lane's row's 16 columns from c on. more: there are 16 others behind them.
+    template <int ACT, typename TOut>
+    __device__ __forceinline__ void block(const ActParams& p, uint8_t* mem, int c, const float (&v)[16], bool more) {
+        const int lane = threadIdx.x & 31, unit = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            *reinterpret_cast<float4*>(mem + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        __syncwarp();
+        const int from = (c >> 2) + unit;                         // the lane that has these columns' bias
+        const float4 b = make_float4(__shfl_sync(0xffffffffu, bias.x, from), __shfl_sync(0xffffffffu, bias.y, from),
+                                     __shfl_sync(0xffffffffu, bias.z, from), __shfl_sync(0xffffffffu, bias.w, from));
+        float x[16];
+        float4 now[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int row = 8 * i + (lane >> 2);
+            const float4 z = *reinterpret_cast<const float4*>(mem + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4));
+            x[4 * i] = z.x + b.x; x[4 * i + 1] = z.y + b.y; x[4 * i + 2] = z.z + b.z; x[4 * i + 3] = z.w + b.w;
+            now[i] = add[i];
+        }
+        const Four here = f;
+        f.at += 16;
+        f.left -= 16;
+        f.live = f.left > 0 ? rows : 0u;
+        if (p.residual && more) residual_of(p, f, add);
+        finish_four<ACT, TOut>(p, here, x, now);
+        __syncwarp();                                             // the block has been read
+    }
+};
+
 // S: slices of K (a cluster of 2 S CTAs, one tile); 1: the pairs walk over the tiles. SUMS: sums in registers (always with slices).
-template <int S, bool SUMS, typename TOut>
+// ACT: with sums of whole tiles the finishing code is there once for every 16 of a thread's columns, for one activation (for all of them it did
+// not fit the instruction cache: 40,000 cycles a tile, and with the sums moved down in a loop they left the registers: 100,000); -1: any.
+template <int S, bool SUMS, int ACT, typename TOut>
 __global__ void __launch_bounds__(NUM_THREADS)
 act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, const ActParams p) {
     static_assert(S == 1 || SUMS, "slices are added in registers");
@@ -193,6 +256,15 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     if (warp == 0) {
         // ---------------------------------------------------------------- TMA producer (of each CTA)
         if (lane == 0) {
+            // The first stages' weights set out before the wait: no kernel writes them.
+            const int pre = walker < n_tiles ? min(STAGES, (n_kb + 1) / 2) : 0;
+            for (int i = 0; i < pre; i++) {
+                const int kb = kb0 + 2 * i, n = min(2, kb1 - kb);
+                if (rank == 0) mbar_expect_tx(full_bar(i), uint32_t(2 * n * (A_BYTES + b_bytes)));
+                for (int j = 0; j < n; j++)
+                    load_tile(base + i * STAGE_BYTES + 2 * A_BYTES + j * B_BYTES, &tm_b, map_cluster(full_bar(i), lead), (kb + j) * BK,
+                              (walker / p.tiles_m) * p.width + int(rank) * b_rows);
+            }
             ib::pdl_wait();
             int it = 0, s = 0;
             uint32_t parity = 1;                                  // of the wait for the slot's use before
@@ -206,12 +278,12 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                     if (slots[1]) break;
                     const uint32_t a_dst = base + s * STAGE_BYTES, b_dst = a_dst + 2 * A_BYTES;
                     const uint32_t bar = map_cluster(full_bar(s), lead);
-                    if (rank == 0) mbar_expect_tx(full_bar(s), uint32_t(2 * n * (A_BYTES + b_bytes)));
+                    if (rank == 0 && it >= pre) mbar_expect_tx(full_bar(s), uint32_t(2 * n * (A_BYTES + b_bytes)));
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
                         if (j < n) {
                             load_tile(a_dst + j * A_BYTES, &tm_a, bar, (kb + j) * BK, a_row);
-                            load_tile(b_dst + j * B_BYTES, &tm_b, bar, (kb + j) * BK, b_row);
+                            if (it >= pre) load_tile(b_dst + j * B_BYTES, &tm_b, bar, (kb + j) * BK, b_row);
                         }
                     }
                     if (++s == STAGES) { s = 0; parity ^= 1u; }
@@ -267,13 +339,15 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     } else {
         // ---------------------------------------------------------------- epilogue: a row of the CTA and half of the columns a thread
         const int quad = warp & 3, half = (warp - 2) >> 2, cols = p.width / 2, c_first = half * cols;
-        const int r = quad * 32 + lane;
+        uint8_t* block = base_ptr + STAGES * STAGE_BYTES + BARS_BYTES + (warp - 2) * BLOCK_BYTES;
         const uint32_t lanes = tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(c_first);
         ib::pdl_wait();
         int use = 0;
         bool ok = true;
         for (int tile = walker; tile < n_tiles && ok; tile += walkers) {
-            const int64_t m = int64_t(tile % p.tiles_m) * (2 * BM) + int64_t(rank) * BM + r, n0 = int64_t(tile / p.tiles_m) * p.width + c_first;
+            const int64_t m0 = int64_t(tile % p.tiles_m) * (2 * BM) + int64_t(rank) * BM + quad * 32, n0 = int64_t(tile / p.tiles_m) * p.width + c_first;
+            TileEnd end;
+            if (S == 1) end.open(p, m0, n0);
             if constexpr (SUMS) {
 #pragma unroll
                 for (int c = 0; c < COLS; c++) acc[c] = 0.0f;
@@ -298,9 +372,8 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
 #pragma unroll 1
                     for (int c = 0; c < cols; c += 16) {
                         float v[16];
-                        __syncwarp();
                         tmem_get16(lanes + uint32_t(b * 256 + c), v);
-                        finish<TOut, 16>(p, m, n0 + c, v);
+                        end.block<ACT, TOut>(p, block, c, v, c + 16 < cols);
                     }
                 }
                 tc_fence_before();
@@ -314,7 +387,7 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                         float v[16];
 #pragma unroll
                         for (int j = 0; j < 16; j++) v[j] = acc[c + j];
-                        finish<TOut, 16>(p, m, n0 + c, v);
+                        end.block<ACT, TOut>(p, block, c, v, c + 16 < cols);
                     }
                 }
             }
@@ -323,31 +396,67 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     }
     if constexpr (S > 1) {
         cluster_sync();                                  // every MMA of the cluster is done: the rings are free
-        // [slice][group of four columns][row][4] of the columns that this CTA owns: width / S from width / S * slice on
+        // [slice][group of four columns][row][4] of the columns that this CTA owns: width / S from width / S * slice on (32 bytes behind each
+        // group: lanes that read two rows of four groups do not meet in a bank)
         const int own = p.width / S, quad = warp & 3, r = quad * 32 + lane, half = (warp - 2) >> 2, cols = p.width / 2;
         if (warp >= 2 && !slots[1]) {
+            int owner = half * cols / own, at = half * cols - owner * own;              // (carried along: no division for each column)
+            uint32_t to = map_cluster(base, uint32_t(owner * 2) + rank);
 #pragma unroll
             for (int c = 0; c < COLS; c += 4) {
                 if (c < cols) {
-                    const int col = half * cols + c, owner = col / own, at = col - owner * own;
-                    const uint32_t to = map_cluster(base + uint32_t(((slice * (own >> 2) + (at >> 2)) * BM + r) * 16), uint32_t(owner * 2) + rank);
-                    st_cluster_v4(to, &acc[c]);
+                    st_cluster_v4(to + uint32_t((slice * (own >> 2) + (at >> 2)) * GROUP_BYTES + r * 16), &acc[c]);
+                    at += 4;
+                    if (at == own) { at = 0; owner++; if (owner < S) to = map_cluster(base, uint32_t(owner * 2) + rank); }
                 }
             }
         }
+        // A warp finishes 8 rows x 4 groups of columns at a time: rows 8 (warp - 2) + 64 h on, h = 0, 1, of the columns 16 q on; four q are a batch.
+        // What is added to the first two batches is requested before the barrier.
+        const int groups = own >> 2, per_h = (groups + 15) >> 4, batches = 2 * per_h;     // (S = 2: up to 4, S = 4: 2)
+        const int64_t n0 = int64_t(walker / p.tiles_m) * p.width + own * slice;
+        auto rows_of = [&](int k) { return 8 * (warp - 2) + (lane >> 2) + (k >= per_h ? 64 : 0); };
+        auto first_of = [&](int k) { return (k >= per_h ? k - per_h : k) * 16 + (lane & 3); };         // group of the batch's first four columns; 4 on: the next
+        auto four_of = [&](int k) {
+            const int64_t m = int64_t(walker % p.tiles_m) * (2 * BM) + int64_t(rank) * BM + rows_of(k), n = n0 + 4 * first_of(k);
+            Four f{m * p.N + n, 16, int(p.N - n), 16, 0u};
+#pragma unroll
+            for (int j = 0; j < 4; j++) f.live |= m < p.M && first_of(k) + 4 * j < groups && n + 16 * j < p.N ? 1u << j : 0u;
+            return f;
+        };
+        auto request = [&](int k, float4 (&bias)[4], float4 (&add)[4]) {
+            const Four f = four_of(k);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                bias[j] = bias_of(p, f.live >> j & 1 ? n0 + 4 * first_of(k) + 16 * j : p.N);
+                add[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+            if (p.residual) residual_of(p, f, add);
+        };
+        float4 bias[2][4], add[2][4];
+        if (warp >= 2) { request(0, bias[0], add[0]); request(1, bias[1], add[1]); }
         __syncwarp();
         cluster_sync();                                  // every slice's columns have arrived
         if (warp >= 2 && !slots[1]) {
-            const int64_t m = int64_t(walker % p.tiles_m) * (2 * BM) + int64_t(rank) * BM + r, n0 = int64_t(walker / p.tiles_m) * p.width + own * slice;
-            const float4* got = reinterpret_cast<const float4*>(base_ptr) + r;
-            for (int g = half; g < own >> 2; g += 2) {
-                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int z = 0; z < S; z++) {
-                    const float4 f = got[(z * (own >> 2) + g) * BM];
-                    v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
+            for (int k = 0; k < (S == 2 ? 4 : 2); k++) {
+                if (k >= batches) break;
+                const Four f = four_of(k);
+                float v[16];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    float4 z = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (f.live >> j & 1) {
+#pragma unroll
+                        for (int o = 0; o < S; o++) {
+                            const float4 g = *reinterpret_cast<const float4*>(base_ptr + (o * groups + first_of(k) + 4 * j) * GROUP_BYTES + rows_of(k) * 16);
+                            z.x += g.x; z.y += g.y; z.z += g.z; z.w += g.w;
+                        }
+                    }
+                    v[4 * j] = z.x + bias[k & 1][j].x; v[4 * j + 1] = z.y + bias[k & 1][j].y; v[4 * j + 2] = z.z + bias[k & 1][j].z; v[4 * j + 3] = z.w + bias[k & 1][j].w;
                 }
-                finish<TOut, 4>(p, m, n0 + 4 * g, v);
+                finish_four<ACT, TOut>(p, f, v, add[k & 1]);
+                if (k + 2 < batches) request(k + 2, bias[k & 1], add[k & 1]);
             }
         }
     }
@@ -361,9 +470,9 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
 }
 
 // Clusters of 2 S CTAs that run at once (at most one CTA an SM).
-template <int S, bool SUMS, typename TOut> int clusters_at_once(int sms) {
+template <int S, bool SUMS, int ACT, typename TOut> int clusters_at_once(int sms) {
     static ib::PerDevice allowed, fit;
-    if (ib::allow_smem(allowed, "linear_act", act_pair_kernel<S, SUMS, TOut>, SMEM_BYTES)) return 0;
+    if (ib::allow_smem(allowed, "linear_act", act_pair_kernel<S, SUMS, ACT, TOut>, SMEM_BYTES)) return 0;
     return fit.get(ib::current_device(), [&] {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(unsigned(sms / (2 * S) * (2 * S)));
@@ -375,31 +484,41 @@ template <int S, bool SUMS, typename TOut> int clusters_at_once(int sms) {
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
         int clusters = 0;
-        const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, act_pair_kernel<S, SUMS, TOut>, &cfg);
+        const cudaError_t e = cudaOccupancyMaxActiveClusters(&clusters, act_pair_kernel<S, SUMS, ACT, TOut>, &cfg);
         return e != cudaSuccess ? 0 : clusters < sms / (2 * S) ? clusters : sms / (2 * S);
     });
 }
 
-template <int S, bool SUMS, typename TOut>
+template <int S, bool SUMS, int ACT, typename TOut>
 int launch_act(const CUtensorMap& ma, const CUtensorMap& mb, const ActParams& p, int sms, cudaStream_t stream) {
-    const int room = clusters_at_once<S, SUMS, TOut>(sms);
+    const int room = clusters_at_once<S, SUMS, ACT, TOut>(sms);
     if (room < 1) return ib::fail(IB_ERR_CUDA, "linear_act: no room for a cluster of %d CTAs", 2 * S);
     const int tiles = p.tiles_m * p.tiles_n;
-    return ib::launch("linear_act", act_pair_kernel<S, SUMS, TOut>, dim3(unsigned(2 * S * (S > 1 || tiles < room ? tiles : room))), dim3(NUM_THREADS),
+    return ib::launch("linear_act", act_pair_kernel<S, SUMS, ACT, TOut>, dim3(unsigned(2 * S * (S > 1 || tiles < room ? tiles : room))), dim3(NUM_THREADS),
                       size_t(SMEM_BYTES), stream, unsigned(2 * S), ma, mb, p);
 }
 
 template <typename TOut> int launch_any(int slices, bool sums, const CUtensorMap& ma, const CUtensorMap& mb, const ActParams& p, int sms, cudaStream_t stream) {
-    if (slices == 4) return launch_act<4, true, TOut>(ma, mb, p, sms, stream);
-    if (slices == 2) return launch_act<2, true, TOut>(ma, mb, p, sms, stream);
-    return sums ? launch_act<1, true, TOut>(ma, mb, p, sms, stream) : launch_act<1, false, TOut>(ma, mb, p, sms, stream);
+    if (slices == 4) return launch_act<4, true, -1, TOut>(ma, mb, p, sms, stream);
+    if (slices == 2) return launch_act<2, true, -1, TOut>(ma, mb, p, sms, stream);
+    if constexpr (sizeof(TOut) == 4) {
+        if (sums) switch (p.act) {
+            case ib::score::NONE: return launch_act<1, true, ib::score::NONE, TOut>(ma, mb, p, sms, stream);
+            case ib::score::RELU: return launch_act<1, true, ib::score::RELU, TOut>(ma, mb, p, sms, stream);
+            case ib::score::RELU_SQUARED: return launch_act<1, true, ib::score::RELU_SQUARED, TOut>(ma, mb, p, sms, stream);
+            case ib::score::GELU_TANH: return launch_act<1, true, ib::score::GELU_TANH, TOut>(ma, mb, p, sms, stream);
+            case ib::score::GELU: return launch_act<1, true, ib::score::GELU, TOut>(ma, mb, p, sms, stream);
+            default: return launch_act<1, true, ib::score::SILU, TOut>(ma, mb, p, sms, stream);
+        }
+    }
+    return launch_act<1, false, -1, TOut>(ma, mb, p, sms, stream);
 }
 
 }  // namespace
 
 // Width of a tile (32 .. 256, a multiple of 32) and slices of K (1, 2 or 4) for a product; sms: of the device. Cycles that a launch takes: rounds x
 // (k-blocks of a slice x (361 + 1.1 width) + what follows the last MMA), with that for a whole tile's epilogue 2,000 + 8 width, for
-// slices 5,000 beside their own columns'.
+// slices 13,000 beside their own columns' (two barriers, the push, another start).
 IB_EXPORT int ib_linear_act_plan(int64_t M, int64_t N, int64_t K, int sms, int* width, int* slices) {
     if (M <= 0 || N <= 0 || K <= 0 || K % 8) return ib::fail(IB_ERR_ARG, "linear_act: sizes must be positive, K a multiple of 8");
     if (M >= (1LL << 30) || N >= (1LL << 30) || K >= (1LL << 30)) return ib::fail(IB_ERR_ARG, "linear_act: a size exceeds 2^30");
@@ -414,7 +533,7 @@ IB_EXPORT int ib_linear_act_plan(int64_t M, int64_t N, int64_t K, int sms, int* 
             const int64_t tiles = tm * ((N + w - 1) / w);
             if (tiles >= (1LL << 28) || (s > 1 && tiles > 2 * room)) continue;
             const int64_t rounds = (tiles + room - 1) / room;
-            const int64_t cost = s == 1 ? rounds * kb * (361 + 11 * w / 10) + 2000 + 8 * w : rounds * ((kb + s - 1) / s * (361 + 11 * w / 10) + 5000 + 8 * w / s);
+            const int64_t cost = s == 1 ? rounds * kb * (361 + 11 * w / 10) + 2000 + 8 * w : rounds * ((kb + s - 1) / s * (361 + 11 * w / 10) + 13000 + 8 * w / s);
             if (least < 0 || cost < least) { least = cost; *width = w; *slices = s; }
         }
     }
@@ -439,13 +558,12 @@ IB_EXPORT int ib_linear_act(const void* x, const void* w, const float* bias, con
     if (tm * tn >= (1LL << 28)) return ib::fail(IB_ERR_ARG, "linear_act: too many tiles");
     p.width = width; p.tiles_m = int(tm); p.tiles_n = int(tn); p.slices = slices;
     p.act = act; p.bias = bias; p.residual = residual; p.out = out; p.status = status;
-    p.vec = N % (out_dtype == IB_F32 ? 4 : 8) == 0 && ((uintptr_t(out) | uintptr_t(residual)) & 15) == 0;
+    p.vec = N % 4 == 0 && (uintptr_t(out) & (out_dtype == IB_F32 ? 15 : 7)) == 0 && (uintptr_t(residual) & 15) == 0;
     CUtensorMap ma, mb;
     int rc = ib::get_map(x, M, K, BM, &ma);
     if (rc) return rc;
     rc = ib::get_map(w, N, K, width / 2, &mb);
     if (rc) return rc;
-    // (float results of up to 512 elements of K are one chain either way)
     if (out_dtype == IB_F32) return launch_any<float>(slices, p.n_kb > CHAIN, ma, mb, p, sms, stream);
     if (out_dtype == IB_BF16) return launch_any<bf16>(slices, false, ma, mb, p, sms, stream);
     return ib::fail(IB_ERR_ARG, "linear_act: unknown output dtype %d", out_dtype);

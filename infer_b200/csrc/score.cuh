@@ -122,17 +122,21 @@ __device__ __forceinline__ uint32_t key_id(unsigned long long k) { return 0xffff
 constexpr int ACTIVATIONS = 6;
 enum { NONE = 0, RELU = 1, RELU_SQUARED = 2, GELU_TANH = 3, GELU = 4, SILU = 5 };
 
-// x sigmoid(y) without an IEEE division: for y below about -88 the exponential is infinite and the quotient 0.
-__device__ __forceinline__ float times_sigmoid(float x, float y) { return __fdividef(x, 1.0f + exp2_fast(-LOG2E * y)); }
+// x sigmoid(y ln 2) without an IEEE division: where 2^-y is infinite the quotient is 0.
+__device__ __forceinline__ float times_sigmoid2(float x, float y) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + exp2_fast(-y)));
+    return x * r;
+}
 
 __device__ __forceinline__ float activate(float z, int act) {
     switch (act) {
         case RELU: return z > 0.0f ? z : (z != z ? z : 0.0f);
         case RELU_SQUARED: { const float r = z > 0.0f ? z : (z != z ? z : 0.0f); return r * r; }
-        // 0.5 z (1 + tanh u) = z sigmoid(2 u), u = sqrt(2/pi) (z + 0.044715 z^3)
-        case GELU_TANH: return times_sigmoid(z, 1.5957691216057308f * fmaf(0.044715f * z * z, z, z));
+        // 0.5 z (1 + tanh u) = z sigmoid(2 u), u = sqrt(2/pi) (z + 0.044715 z^3); the constants are 2 sqrt(2/pi) log2(e) and 0.044715 of it
+        case GELU_TANH: return times_sigmoid2(z, z * fmaf(z * z, 0.10294324f, 2.3022082f));
         case GELU: return 0.5f * z * erfcf(-0.70710678118654752f * z);
-        case SILU: return times_sigmoid(z, z);
+        case SILU: return times_sigmoid2(z, LOG2E * z);
     }
     return z;
 }
