@@ -9,13 +9,13 @@ __version__ = "0.1.0"
 
 def __getattr__(name):
     # Lazy, so that importing the package (for the configuration or the cache manager alone) does not load torch kernels.
-    if name in ("LLM", "GenerationEngine"):
+    if name in ("LLM", "GenerationEngine", "PromptScore"):
         from .engine import generation
         return getattr(generation, name)
     if name in ("Engine", "StepEntry"):
         from . import engine
         return getattr(engine, name)
-    if name in ("Request", "SampleParams", "Scheduler", "SchedulerConfig", "Completed", "StopReason"):
+    if name in ("Request", "SampleParams", "Scheduler", "SchedulerConfig", "Completed", "StopReason", "TokenScore"):
         from .engine import scheduler
         return getattr(scheduler, name)
     raise AttributeError(name)

@@ -43,6 +43,9 @@ def main(argv=None) -> int:
     ap.add_argument("--weights-seed", type=int, default=0, help="seed of the random weights (--random)")
     ap.add_argument("--kv-blocks", type=int, default=0, help="pages of 16 positions in the cache pool (0: max-seq positions)")
     ap.add_argument("--chunk", type=int, default=512, help="most prompt tokens a step takes")
+    ap.add_argument("--logprobs", type=int, default=None, metavar="N", help="a line for each new token: its log probability, the entropy and the N likeliest "
+                    "tokens (0 to 20; with the cache on)")
+    ap.add_argument("--score", action="store_true", help="also print how likely the model finds the prompt itself")
     args = ap.parse_args(argv)
     names = ["prompt", "n_new", "device", "gemm", "cache", "attn", "step"]
     opt = {"prompt": "0", "n_new": "16", "device": "gpu", "gemm": "mine", "cache": "on", "attn": "split", "step": "fused"}
@@ -99,6 +102,7 @@ def main(argv=None) -> int:
         pi = int(opt["prompt"])
         n = args.prompt_len or 5 + 7 * pi
         ids = np.random.default_rng(pi).integers(0, V, n).tolist()
+    scores = ()
     print(f"model {args.model}")
     print(f"prompt {opt['prompt']} ({len(ids)} tokens), device=gpu gemm={opt['gemm']} cache={opt['cache']} "
           f"attn={opt['attn']} step={opt['step']} dtype={args.dtype}:")
@@ -124,10 +128,17 @@ def main(argv=None) -> int:
         stamps = []
         t0 = time.perf_counter()
         out = llm.generate([ids], max_new=n_new, temperature=args.temp, seed=args.seed, top_k=args.top_k,
-                           top_p=args.top_p, on_token=lambda rid, tok: stamps.append(time.perf_counter()))[0]
+                           top_p=args.top_p, on_token=lambda rid, tok: stamps.append(time.perf_counter()), logprobs=args.logprobs)[0]
+        if args.logprobs is not None:
+            out, scores = out
         total = time.perf_counter() - t0
         t_first = (stamps[0] - t0) if stamps else total
     print("ids:", " ".join(str(t) for t in out))
+    for tok, s in zip(out, scores):
+        print(f"token {tok} logprob {s.logprob:.4f} entropy {s.entropy:.4f}" + "".join(f" {t}:{p:.4f}" for t, p in s.top))
+    if args.score:
+        s = llm.score([ids])[0]
+        print(f"prompt logprob {float(s.logprobs.sum()):.4f} perplexity {s.perplexity:.3f} entropy {float(s.entropies.mean()) if len(s.entropies) else 0.0:.4f}")
     rest = max(1e-9, total - t_first)
     print(f"prefill {t_first:.4f} s, decode {max(0, len(out) - 1) / rest:.1f} tok/s ({len(out)} tokens, {total:.3f} s)")
     return 0

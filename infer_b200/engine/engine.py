@@ -484,6 +484,16 @@ class Engine:
         Raises OutOfPages (nothing changed) if the pages for all entries together are not free."""
         return self._step(entries, sample, False).output
 
+    def step_logprobs(self, entries: Sequence[StepEntry], tokens: Sequence[int], top: int = 0) -> "ops.TokenLogprobs":
+        """As ``step``, but in place of logits it returns how likely ``tokens`` (one id per wanted place, in the order of the entries and of
+        their ``want`` lists; -1: none) are there, the entropy at each place and the ``top`` likeliest tokens, on the device
+        (``ops.token_logprobs`` says exactly what). The logits are not stored, so that every place of a long portion may be wanted."""
+        tokens = [int(t) for t in tokens]
+        bad = [t for t in tokens if not -1 <= t < self.spec.vocab_size]
+        if bad:
+            raise ValueError(f"token id {bad[0]} is outside the vocabulary [0, {self.spec.vocab_size})")
+        return self._step(entries, None, False, (tokens, top)).output
+
     def try_step(self, entries: Sequence[StepEntry], sample=None) -> StepResult:
         """As ``step``, but an entry that cannot get its pages (after the entries before it have taken theirs) or
         that would pass the sequence limit is left out instead of failing the call: the others run, the result says
@@ -491,10 +501,19 @@ class Engine:
         kernels/batch_gpu.cu:386-410). ``sample`` still has one item per wanted place of ALL entries."""
         return self._step(entries, sample, True)
 
-    def _step(self, entries, sample, partial: bool) -> StepResult:
+    def _step(self, entries, sample, partial: bool, score=None) -> StepResult:
+        """``score``: (a token id per wanted place, how many alternatives), for ``step_logprobs``; such a step runs eagerly."""
         entries = [e if isinstance(e, StepEntry) else StepEntry(*e) for e in entries]
         empty_dtype = torch.int32 if sample is not None else torch.float32
         empty_shape = (0,) if sample is not None else (0, self.spec.vocab_size)
+        if score is not None:
+            n_want = sum(len(e.want) for e in entries)
+            if len(score[0]) != n_want:
+                raise ValueError(f"one token id per wanted place: {len(score[0])} given, {n_want} wanted")
+            with torch.cuda.device(self.rt.device):
+                asked = torch.tensor(score[0], dtype=torch.int32).pin_memory().to(self.rt.device, non_blocking=True)
+                if not entries:
+                    return StepResult(ops.token_logprobs(torch.empty(empty_shape, device=self.rt.device), asked, score[1]), [])
         if not entries:
             return StepResult(torch.empty(empty_shape, dtype=empty_dtype, device=self.rt.device), [])
         rids = [e.rid for e in entries]
@@ -529,13 +548,15 @@ class Engine:
                 raise AssertionError("reserve failed after can_reserve succeeded")
         try:
             self._look_at_parts()
-            ctx, entry = self._build_context(entries, self.use_graphs, sample)
+            ctx, entry = self._build_context(entries, self.use_graphs and score is None, sample)
         except Exception:
             for rid, _ in wanted:
                 self.cache.unreserve(rid)
             raise
         with torch.cuda.device(self.rt.device):
-            if entry is None:
+            if score is not None:
+                out = self.model.logprobs(ctx, self.cache_views, asked, score[1])
+            elif entry is None:
                 out = self._run_model(ctx) if ctx.measured is None else self._run_measured(ctx, ctx.measured)
             elif len(entry.graphs) == entry.copies:
                 # Copies of the graph take turns: launching an executable graph again while its previous launch is
@@ -586,6 +607,9 @@ class Engine:
                     102: "a tensor-core GEMM's operand wait ran out", 103: "a tensor-core GEMM's accumulator wait ran out",
                     104: "the streaming product's wait ran out", 106: "the prefill attention's wait ran out",
                     107: "the score attention's wait ran out", 131: "the 32-bit tensor-core product's wait ran out",
+                    141: "a copy wait of the head's log probabilities ran out", 142: "an operand wait of the head's log probabilities ran out",
+                    143: "an accumulator wait of the head's log probabilities ran out", 151: "a copy wait of a product with an activation ran out",
+                    152: "an operand wait of a product with an activation ran out", 153: "an accumulator wait of a product with an activation ran out",
                     108: "the prefill attention's shared memory does not start on a 1024-byte boundary",
                     }.get(code, f"code {code}")
             raise RuntimeError(f"device status word was raised: {what}")

@@ -8,10 +8,11 @@ what the spec lists and calls ``forward`` on the embedding, the blocks, the fina
 from __future__ import annotations
 
 from types import FunctionType
-from typing import Dict, List, Mapping
+from typing import Dict, List, Mapping, Optional
 
 import torch
 
+from .. import ops
 from ..config.specs import LayerSpec, ModelSpec, PartSpec
 from ..parts.base import Block, Part, Watched, build_part, part_class
 from ..parts.linear import Linear
@@ -103,18 +104,30 @@ class Model(Watched):
         return needs
 
     def forward(self, step, cache_views: Mapping[int, object]) -> torch.Tensor:
+        normed = self._wanted_rows(step, cache_views)
+        if normed is None:
+            return torch.empty((0, self.spec.vocab_size), dtype=torch.float32, device=self.rt.device)
+        return self.head.forward(normed)                                           # float32 [wanted, vocab]
+
+    def logprobs(self, step, cache_views: Mapping[int, object], tokens: torch.Tensor, top: int):
+        """``forward``, with how likely ``tokens`` (int32 [wanted]) are at the wanted places in place of logits (``ops.TokenLogprobs``)."""
+        normed = self._wanted_rows(step, cache_views)
+        if normed is None:
+            return ops.token_logprobs(torch.empty((0, self.spec.vocab_size), dtype=torch.float32, device=self.rt.device), tokens, top)
+        return self.head.logprobs(normed, tokens, top, step.status)
+
+    def _wanted_rows(self, step, cache_views: Mapping[int, object]) -> Optional[torch.Tensor]:
+        """The step's tokens through the layers; the wanted places' normalised rows (None: no place is wanted)."""
         h = self.embedding.forward(step)                                           # float32 [T, hidden]
         if self.stream is not None:
             h = self.stream.open(h)
         for call in self.spec.schedule:
             h = self.blocks[call.layer].forward(h, step, cache_views[call.cache], call.write_cache)
         if step.n_want == 0:
-            return torch.empty((0, self.spec.vocab_size), dtype=torch.float32, device=self.rt.device)
+            return None
         if self.stream is not None:
-            normed = self.stream.close(h, self.final_norm, step.want_rows)
-        else:
-            normed = self.final_norm.forward(h, rows=step.want_rows)              # [wanted, hidden]
-        return self.head.forward(normed)                                           # float32 [wanted, vocab]
+            return self.stream.close(h, self.final_norm, step.want_rows)
+        return self.final_norm.forward(h, rows=step.want_rows)                     # [wanted, hidden]
 
     def weight_bytes(self) -> int:
         """Bytes of every distinct parameter tensor on the device (a decode step reads each once)."""

@@ -49,6 +49,16 @@ class SampleParams:
     seed: int = 0
     top_k: int = 0
     top_p: float = 1.0
+    logprobs: Optional[int] = None      # how likely each token was, with so many alternatives (0 to 20), under softmax(logits); None: not asked
+
+
+@dataclass
+class TokenScore:
+    """How likely a generated token was: its log probability, the entropy (nats) of the distribution that it came from, and the
+    likeliest tokens with their log probabilities."""
+    logprob: float
+    entropy: float
+    top: List[Tuple[int, float]] = field(default_factory=list)
 
 
 @dataclass
@@ -60,6 +70,7 @@ class Request:
     sample: SampleParams = field(default_factory=SampleParams)
     eos_id: Optional[int] = USE_DEFAULT_EOS           # None: the scheduler's eos_id; -1: never stop on eos
     generated_so_far: List[int] = field(default_factory=list)   # set by preemption
+    scores_so_far: List[TokenScore] = field(default_factory=list)
 
 
 class StopReason(IntEnum):
@@ -80,6 +91,7 @@ class Completed:
     first_token_ms: float = 0.0
     finished_ms: float = 0.0
     preemptions: int = 0
+    scores: List[TokenScore] = field(default_factory=list)      # one per token, if the request asked for them
 
 
 @dataclass
@@ -191,6 +203,7 @@ class _Active:
     first_token_ms: float = 0.0
     preemptions: int = 0
     pending: int = 0                # tokens sampled on the device that the host has not read yet (overlap mode)
+    scores: List[TokenScore] = field(default_factory=list)
 
     @property
     def decoding(self) -> bool:
@@ -255,7 +268,7 @@ class Scheduler:
         a = self.active.pop(rid)
         self.eng.end_request(rid)
         c = Completed(rid, reason, a.out, a.admitted_step, self._step, a.admitted_ms, a.first_token_ms,
-                      self._now(), a.preemptions)
+                      self._now(), a.preemptions, a.scores)
         self.completed.append(c)
         self._event("retire", rid, reason, tokens=len(c.tokens))
         if self.cfg.on_done:
@@ -264,7 +277,7 @@ class Scheduler:
     def _finish_unstarted(self, r: Request, reason: StopReason) -> None:
         now = self._now()
         c = Completed(r.id, reason, list(r.generated_so_far), self._step, self._step, now, now, now,
-                      self._preempt_counts.get(r.id, 0))
+                      self._preempt_counts.get(r.id, 0), list(r.scores_so_far))
         self.completed.append(c)
         if self.cfg.on_done:
             self.cfg.on_done(c)
@@ -287,7 +300,7 @@ class Scheduler:
             self.eng.add_request(r.id)
             a = _Active(r, list(r.generated_so_far), len(r.prompt) - len(r.generated_so_far),
                         admitted_step=self._step, admitted_seq=self._admit_seq, admitted_ms=self._now(),
-                        preemptions=self._preempt_counts.get(r.id, 0))
+                        preemptions=self._preempt_counts.get(r.id, 0), scores=list(r.scores_so_far))
             self._admit_seq += 1
             self.active[r.id] = a
             self._event("admit", r.id, tokens=len(r.prompt))
@@ -302,6 +315,7 @@ class Scheduler:
         r = a.req
         r.prompt = list(r.prompt) + a.out[len(r.generated_so_far):]
         r.generated_so_far = list(a.out)
+        r.scores_so_far = list(a.scores)
         r.arrival_step = 0
         self._preempt_counts[rid] = a.preemptions + 1
         self.queue.appendleft(r)
@@ -343,8 +357,8 @@ class Scheduler:
             budget -= n
         return batch
 
-    def _take_tokens(self, batch, sampled) -> int:
-        """Appends the sampled tokens to their requests, calls back, and retires what has finished."""
+    def _take_tokens(self, batch, sampled, scores=None) -> int:
+        """Appends the sampled tokens (and their ``scores``, for those that asked) to their requests, calls back, and retires what has finished."""
         decoded = 0
         for b in batch:
             if b.sample is None:
@@ -359,6 +373,8 @@ class Scheduler:
                 a.first_token_ms = self._now()
             a.last_token = tok
             a.out.append(tok)
+            if scores and b.rid in scores:
+                a.scores.append(scores[b.rid])
             decoded += 1
             if self.cfg.on_token:
                 self.cfg.on_token(b.rid, tok)
@@ -377,7 +393,7 @@ class Scheduler:
         self._pending = None
         # a request admitted again after a preemption must not take a token of its earlier life
         live = [b for b in batch if b.rid in self.active and self.active[b.rid].admitted_seq == seqs[b.rid]]
-        return self._take_tokens(live, handle.result())
+        return self._take_tokens(live, handle.result(), getattr(handle, "scores", None))
 
     def step(self) -> int:
         """Cancel -> admit -> plan (preempting while nothing can move) -> run -> retire. Returns tokens decoded."""
@@ -413,12 +429,17 @@ class Scheduler:
             decoded = self._apply_pending()             # the previous step's tokens, while this step runs
             self._pending = launched
         elif batch:
-            sampled = self.eng.run(batch)
+            scores = None
+            if any(b.sample is not None and b.sample.logprobs is not None for b in batch):
+                handle = self.eng.run_async(batch)
+                sampled, scores = handle.result(), getattr(handle, "scores", None)
+            else:
+                sampled = self.eng.run(batch)
             for b in batch:
                 a = self.active[b.rid]
                 if not a.decoding:
                     a.fed += len(b.tokens)
-            decoded = self._take_tokens(batch, sampled)
+            decoded = self._take_tokens(batch, sampled, scores)
         self._event("step", tokens=n_tokens, decoded=decoded, t=t_start, dur=self._now() - t_start)
         self._step += 1
         return decoded

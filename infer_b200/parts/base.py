@@ -256,6 +256,12 @@ class Embedding(Part):
 class Head(Part):
     """Normalised rows -> float32 logits [rows, vocab]."""
 
+    def logprobs(self, x: torch.Tensor, tokens: Optional[torch.Tensor], top: int, status: Optional[torch.Tensor] = None):
+        """How likely ``tokens`` (int32 [rows]) are behind the rows x, and the ``top`` likeliest (``ops.TokenLogprobs``): of this head's logits.
+        A head that need not store them says so in a method of its own."""
+        from .. import ops
+        return ops.token_logprobs(self.forward(x), tokens, top, status)
+
     def tie(self, embedding: Embedding) -> None:
         """Called once after loading, with the model's embedding part; a tied head takes its matrix from there."""
 

@@ -53,15 +53,19 @@ class Linear(Watched):
         return cls(rt, torch.cat(mats, dim=0), torch.cat(biases) if any_bias else None), starts
 
     def __call__(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None,
-                 out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                 out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None, activation: Optional[str] = None) -> torch.Tensor:
         """x [rows, in] in the compute dtype (or a DeferredNorm of float32 rows). With ``residual`` (float32 [rows, out]) the result is
         float32 and is written over ``residual``. Otherwise the result has ``out_dtype`` (default:
-        the compute dtype), and is written into ``out`` (contiguous [rows, out] of that dtype) if given."""
+        the compute dtype), and is written into ``out`` (contiguous [rows, out] of that dtype) if given. ``activation``: of the product and its
+        bias, before the residual, without a rounding between (``ops.linear_act`` names them)."""
         from .base import DeferredNorm
         if residual is not None:
             out, out_dtype = residual, torch.float32
         elif out is not None:
             out_dtype = out.dtype
+        if activation is not None:
+            x = x.materialize() if isinstance(x, DeferredNorm) else x
+            return ops.linear_act(x, self.weight, self.bias, activation, residual, out_dtype or self.rt.dtype, out)
         if self.rt.fast("linear"):
             from .. import fast_ops
             y = fast_ops.linear(x, self.weight, self.bias, residual, out_dtype or self.rt.dtype, out)

@@ -107,6 +107,13 @@ class LinearHead(Head):
             raise ValueError("a tied head needs an embedding part with a [vocab, hidden] table")
         self.linear = Linear.share(self.rt, table)
 
+    def logprobs(self, x, tokens, top, status=None):
+        # (a subclass or an instance with logits of its own goes by those)
+        if type(self).forward is not LinearHead.forward or "forward" in vars(self) or type(self.linear) is not Linear or self.linear.bias is not None \
+                or not self.rt.fast("linear"):
+            return super().logprobs(x, tokens, top, status)
+        return ops.head_logprobs(x, self.linear.weight, tokens, top, self.logit_scale, self.softcap, status)
+
     def forward(self, x):
         logits = self.linear(x, out_dtype=torch.float32)
         if self.logit_scale != 1.0 or self.softcap > 0:
