@@ -88,6 +88,7 @@ __device__ __forceinline__ void tmem_get16(uint32_t taddr, float (&v)[16]) {
 struct ActParams {
     int64_t M, N;
     int n_kb, width, tiles_m, tiles_n, slices;
+    int a_rows;                  // rows of a CTA, up to 128: dealt out evenly, since copies that reach behind the last row take far longer
     int act, vec;                // vec: four columns of out (16 or 8 bytes) and residual (16) start on such a boundary
     const float* bias;           // [N] or null
     const float* residual;       // [M, N] or null (may be out)
@@ -162,7 +163,7 @@ struct TileEnd {
     Four f;                      // of the tile's first 16 columns
     uint32_t rows;
     float4 bias, add[4];         // bias: of columns 4 lane on
-    __device__ __forceinline__ void open(const ActParams& p, int64_t m0, int64_t n0) {
+    __device__ __forceinline__ void open(const ActParams& p, int64_t m0, int64_t m_end, int64_t n0) {
         const int lane = threadIdx.x & 31, unit = lane & 3;
         const int64_t m = m0 + (lane >> 2);
         f.at = m * p.N + n0 + 4 * unit;
@@ -171,7 +172,7 @@ struct TileEnd {
         f.less = 0;
         rows = 0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) rows |= m + 8 * i < p.M ? 1u << i : 0u;
+        for (int i = 0; i < 4; i++) rows |= m + 8 * i < m_end ? 1u << i : 0u;
         f.live = f.left > 0 ? rows : 0u;
         bias = bias_of(p, n0 + 4 * lane);
 #pragma unroll
@@ -227,7 +228,7 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     const int walker = blockIdx.x / (2 * S), walkers = gridDim.x / (2 * S), n_tiles = p.tiles_m * p.tiles_n;
     const int kb0 = int(int64_t(slice) * ((p.n_kb + 1) / 2) / S) * 2, kb1 = min(p.n_kb, int(int64_t(slice + 1) * ((p.n_kb + 1) / 2) / S) * 2);
     const int n_kb = kb1 - kb0, chains = SUMS ? (n_kb + CHAIN - 1) / CHAIN : 1;
-    const int b_rows = p.width / 2, b_bytes = b_rows * BK * 2;
+    const int b_rows = p.width / 2, a_bytes = p.a_rows * BK * 2, b_bytes = b_rows * BK * 2;
     auto full_bar = [&](int s) { return bars + 8u * s; };
     auto empty_bar = [&](int s) { return bars + 8u * (STAGES + s); };
     auto acc_full_bar = [&](int b) { return bars + 8u * (2 * STAGES + b); };
@@ -260,7 +261,7 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
             const int pre = walker < n_tiles ? min(STAGES, (n_kb + 1) / 2) : 0;
             for (int i = 0; i < pre; i++) {
                 const int kb = kb0 + 2 * i, n = min(2, kb1 - kb);
-                if (rank == 0) mbar_expect_tx(full_bar(i), uint32_t(2 * n * (A_BYTES + b_bytes)));
+                if (rank == 0) mbar_expect_tx(full_bar(i), uint32_t(2 * n * (a_bytes + b_bytes)));
                 for (int j = 0; j < n; j++)
                     load_tile(base + i * STAGE_BYTES + 2 * A_BYTES + j * B_BYTES, &tm_b, map_cluster(full_bar(i), lead), (kb + j) * BK,
                               (walker / p.tiles_m) * p.width + int(rank) * b_rows);
@@ -269,7 +270,7 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
             int it = 0, s = 0;
             uint32_t parity = 1;                                  // of the wait for the slot's use before
             for (int tile = walker; tile < n_tiles && !slots[1]; tile += walkers) {
-                const int a_row = (tile % p.tiles_m) * (2 * BM) + int(rank) * BM, b_row = (tile / p.tiles_m) * p.width + int(rank) * b_rows;
+                const int a_row = ((tile % p.tiles_m) * 2 + int(rank)) * p.a_rows, b_row = (tile / p.tiles_m) * p.width + int(rank) * b_rows;
                 for (int kb = kb0; kb < kb1; kb += 2, it++) {
                     const int n = min(2, kb1 - kb);
                     if (it >= STAGES && !mbar_wait(empty_bar(s), parity)) {
@@ -278,7 +279,7 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                     if (slots[1]) break;
                     const uint32_t a_dst = base + s * STAGE_BYTES, b_dst = a_dst + 2 * A_BYTES;
                     const uint32_t bar = map_cluster(full_bar(s), lead);
-                    if (rank == 0 && it >= pre) mbar_expect_tx(full_bar(s), uint32_t(2 * n * (A_BYTES + b_bytes)));
+                    if (rank == 0 && it >= pre) mbar_expect_tx(full_bar(s), uint32_t(2 * n * (a_bytes + b_bytes)));
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
                         if (j < n) {
@@ -345,9 +346,9 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
         int use = 0;
         bool ok = true;
         for (int tile = walker; tile < n_tiles && ok; tile += walkers) {
-            const int64_t m0 = int64_t(tile % p.tiles_m) * (2 * BM) + int64_t(rank) * BM + quad * 32, n0 = int64_t(tile / p.tiles_m) * p.width + c_first;
+            const int64_t m_cta = int64_t((tile % p.tiles_m) * 2 + int(rank)) * p.a_rows, m0 = m_cta + quad * 32, m_end = min(p.M, m_cta + p.a_rows), n0 = int64_t(tile / p.tiles_m) * p.width + c_first;
             TileEnd end;
-            if (S == 1) end.open(p, m0, n0);
+            if (S == 1) end.open(p, m0, m_end, n0);
             if constexpr (SUMS) {
 #pragma unroll
                 for (int c = 0; c < COLS; c++) acc[c] = 0.0f;
@@ -418,10 +419,10 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
         auto rows_of = [&](int k) { return 8 * (warp - 2) + (lane >> 2) + (k >= per_h ? 64 : 0); };
         auto first_of = [&](int k) { return (k >= per_h ? k - per_h : k) * 16 + (lane & 3); };         // group of the batch's first four columns; 4 on: the next
         auto four_of = [&](int k) {
-            const int64_t m = int64_t(walker % p.tiles_m) * (2 * BM) + int64_t(rank) * BM + rows_of(k), n = n0 + 4 * first_of(k);
+            const int64_t m = int64_t((walker % p.tiles_m) * 2 + int(rank)) * p.a_rows + rows_of(k), n = n0 + 4 * first_of(k);
             Four f{m * p.N + n, 16, int(p.N - n), 16, 0u};
 #pragma unroll
-            for (int j = 0; j < 4; j++) f.live |= m < p.M && first_of(k) + 4 * j < groups && n + 16 * j < p.N ? 1u << j : 0u;
+            for (int j = 0; j < 4; j++) f.live |= rows_of(k) < p.a_rows && m < p.M && first_of(k) + 4 * j < groups && n + 16 * j < p.N ? 1u << j : 0u;
             return f;
         };
         auto request = [&](int k, float4 (&bias)[4], float4 (&add)[4]) {
@@ -537,6 +538,9 @@ IB_EXPORT int ib_linear_act_plan(int64_t M, int64_t N, int64_t K, int sms, int* 
             if (least < 0 || cost < least) { least = cost; *width = w; *slices = s; }
         }
     }
+    // (as many tiles, but no wider than they need to be)
+    const int64_t tn = (N + *width - 1) / *width;
+    if (least >= 0) *width = int(((N + tn - 1) / tn + 31) / 32 * 32);
     return least < 0 ? ib::fail(IB_ERR_ARG, "linear_act: too many tiles") : IB_OK;
 }
 
@@ -557,10 +561,11 @@ IB_EXPORT int ib_linear_act(const void* x, const void* w, const float* bias, con
     const int64_t tm = (M + 2 * BM - 1) / (2 * BM), tn = (N + width - 1) / width;
     if (tm * tn >= (1LL << 28)) return ib::fail(IB_ERR_ARG, "linear_act: too many tiles");
     p.width = width; p.tiles_m = int(tm); p.tiles_n = int(tn); p.slices = slices;
+    p.a_rows = int(((M + 2 * tm - 1) / (2 * tm) + 7) / 8 * 8);
     p.act = act; p.bias = bias; p.residual = residual; p.out = out; p.status = status;
     p.vec = N % 4 == 0 && (uintptr_t(out) & (out_dtype == IB_F32 ? 15 : 7)) == 0 && (uintptr_t(residual) & 15) == 0;
     CUtensorMap ma, mb;
-    int rc = ib::get_map(x, M, K, BM, &ma);
+    int rc = ib::get_map(x, M, K, p.a_rows, &ma);
     if (rc) return rc;
     rc = ib::get_map(w, N, K, width / 2, &mb);
     if (rc) return rc;

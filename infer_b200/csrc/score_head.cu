@@ -143,6 +143,9 @@ template <> struct Best<0> {
 struct HeadParams {
     int64_t T, V;
     int n_kb, width, tiles_n, chunks, row_blocks;
+    int a_rows;                  // rows of a CTA, up to 128: dealt out evenly, so that hardly a copy reaches behind the last row (such rows are not only
+                                 // zeros to write: 17 rows in boxes of 128 took 122 us where boxes of 24 take 74; what lies in shared memory
+                                 // behind the loaded rows goes into sums that nobody reads)
     int weights_once;            // the matrix is read once: its tiles leave L2 first
     float scale, cap;
     const int* tokens;           // [T] or null
@@ -166,14 +169,14 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0;
     const int walker = blockIdx.x / CG, walkers = gridDim.x / CG, units = p.row_blocks * p.chunks;
-    const int n_kb = p.n_kb, b_rows = p.width / CG, b_bytes = b_rows * BK * 2;
+    const int n_kb = p.n_kb, b_rows = p.width / CG, a_bytes = p.a_rows * BK * 2, b_bytes = b_rows * BK * 2;
     auto full_bar = [&](int s) { return bars + 8u * s; };
     auto empty_bar = [&](int s) { return bars + 8u * (S + s); };
     auto acc_full_bar = [&](int b) { return bars + 8u * (2 * S + b); };
     auto acc_empty_bar = [&](int b) { return bars + 8u * (2 * S + 2 + b); };
     // CTAs of different chunks go through K from different places on, or all SMs would ask the same few L2 slices for x at a time
     auto first_kb = [&](int chunk) { return int(int64_t(chunk) * ((n_kb + KPS - 1) / KPS) / p.chunks) * KPS; };
-    auto first_tile = [&](int chunk) { return int(int64_t(chunk) * p.tiles_n / p.chunks); };
+    auto tiles_of = [&](int chunk) { return (p.tiles_n - chunk + p.chunks - 1) / p.chunks; };         // tiles chunk, chunk + chunks, ...
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
@@ -207,9 +210,8 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
             uint32_t parity = 1;                                  // of the wait for the slot's use before
             const uint64_t once = policy_evict_first();
             for (int u = walker; u < units && !slots[1]; u += walkers) {
-                const int chunk = u / p.row_blocks, a_row = (u % p.row_blocks) * (BM * CG) + int(rank) * BM;
-                const int t_end = first_tile(chunk + 1);
-                for (int tile = first_tile(chunk); tile < t_end && !slots[1]; tile++) {
+                const int chunk = u / p.row_blocks, a_row = ((u % p.row_blocks) * CG + int(rank)) * p.a_rows;
+                for (int tile = chunk; tile < p.tiles_n && !slots[1]; tile += p.chunks) {
                     const int b_row = tile * p.width + int(rank) * b_rows;
                     for (int i = 0, kb = first_kb(chunk); i < n_kb; i += KPS, kb = kb + KPS < n_kb ? kb + KPS : 0, it++) {
                         const int n = min(KPS, n_kb - kb);
@@ -219,7 +221,7 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                         if (slots[1]) break;
                         const uint32_t a_dst = base + s * R::STAGE_BYTES, b_dst = a_dst + KPS * A_BYTES;
                         const uint32_t bar = CG == 2 ? map_cluster(full_bar(s), 0u) : full_bar(s);
-                        if (rank == 0) mbar_expect_tx(full_bar(s), uint32_t(CG * n * (A_BYTES + b_bytes)));
+                        if (rank == 0) mbar_expect_tx(full_bar(s), uint32_t(CG * n * (a_bytes + b_bytes)));
 #pragma unroll
                         for (int j = 0; j < KPS; j++) {
                             if (j < n) {
@@ -245,7 +247,7 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
             uint32_t parity = 0;
             bool ok = true;
             for (int u = walker; u < units && ok; u += walkers) {
-                const int chunk = u / p.row_blocks, n_tiles = first_tile(chunk + 1) - first_tile(chunk);
+                const int chunk = u / p.row_blocks, n_tiles = tiles_of(chunk);
                 for (int i = 0; i < n_tiles && ok; i++, lt++) {
                     const int b = lt & 1;
                     if (lt >= 2 && !mbar_wait_each(acc_empty_bar(b), ((lt >> 1) - 1) & 1)) { ok = false; break; }      // it has been drained
@@ -282,15 +284,16 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
         int lt = 0;
         bool ok = true;
         for (int u = walker; u < units && ok; u += walkers) {
-            const int chunk = u / p.row_blocks, t_begin = first_tile(chunk), t_end = first_tile(chunk + 1);
-            const int64_t row = int64_t(u % p.row_blocks) * (BM * CG) + int64_t(rank) * BM + quad * 32 + lane;
-            const bool live = row - lane < p.T;                  // (of the warp: some row of it is one)
-            const int token = p.tokens && row < p.T ? p.tokens[row] : -1;
+            const int chunk = u / p.row_blocks;
+            const int64_t row = int64_t((u % p.row_blocks) * CG + int(rank)) * p.a_rows + quad * 32 + lane;
+            const bool live = quad * 32 < p.a_rows && row - lane < p.T;                  // (of the warp: some row of it is one)
+            const bool mine = quad * 32 + lane < p.a_rows && row < p.T;
+            const int token = p.tokens && mine ? p.tokens[row] : -1;
             Stats st;
             st.clear();
             Best<N> best;
             best.clear();
-            for (int tile = t_begin; tile < t_end; tile++, lt++) {
+            for (int tile = chunk; tile < p.tiles_n; tile += p.chunks, lt++) {
                 const int b = lt & 1;
                 ok = __all_sync(0xffffffffu, !slots[1]);
                 if (ok && !mbar_wait_warp(acc_full_bar(b), (lt >> 1) & 1)) { atomicExch(p.status, STATUS_TIMEOUT_EPILOGUE); slots[1] = 1; ok = false; }
@@ -334,7 +337,7 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                     else mbar_arrive(acc_empty_bar(b));
                 }
             }
-            if (ok && row < p.T) {
+            if (ok && mine) {
                 const int64_t at = int64_t(chunk) * p.T + row;
                 p.stats[at] = make_float4(st.m, st.s, st.d, 0.0f);
                 if constexpr (N > 0) {
@@ -375,25 +378,48 @@ struct JoinParams {
     int* status;
 };
 
+// How many of n keys in shared memory are above k.
+__device__ __forceinline__ int beaten_by(const unsigned long long* keys, int n, unsigned long long k) {
+    int above = 0, j = 0;
+    for (; j + 8 <= n; j += 8) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) above += keys[j + e] > k;
+    }
+    for (; j < n; j++) above += keys[j] > k;
+    return above;
+}
+
 __global__ void __launch_bounds__(JOIN_THREADS)
 join_chunks_kernel(const JoinParams p) {
-    extern __shared__ __align__(16) unsigned long long heads[];        // [chunks] first keys, then the survivors
+    extern __shared__ __align__(16) unsigned char join_mem[];
+    float4* stats = reinterpret_cast<float4*>(join_mem);               // [chunks]
+    unsigned long long* heads = reinterpret_cast<unsigned long long*>(stats + p.chunks);        // [chunks] first keys
+    unsigned long long* found = heads + p.chunks;                       // the keys that are compared
     __shared__ unsigned long long bound;
-    __shared__ int n_found;
+    __shared__ int n_found, n_chosen, chosen[MAX_TOP];
     __shared__ Stats total;
     const int64_t row = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (threadIdx.x == 0) { bound = 1; n_found = 0; }
+    if (threadIdx.x == 0) { bound = 1; n_found = n_chosen = 0; }
     ib::pdl_wait();
     ib::pdl_launch_dependents();
+    auto list = [&](int c) { return p.lists + (int64_t(c) * p.T + row) * p.n; };
+    const int token = p.tokens && warp == 0 ? p.tokens[row] : -1;
+    const float at = token >= 0 && token < p.V ? p.at[row] : 0.0f;
+    for (int c = threadIdx.x; c < p.chunks; c += JOIN_THREADS) {        // (everything that is read at first, in one trip to L2)
+        stats[c] = p.stats[int64_t(c) * p.T + row];
+        if (p.top) heads[c] = list(c)[0];
+    }
+    unsigned long long lasts = 1;
+    if (p.top && p.chunks < p.top && warp == 0) for (int c = lane; c < p.chunks; c += 32) lasts = max(lasts, list(c)[p.top - 1]);
+    __syncthreads();
     if (warp == 0) {
         float m = -INFINITY;
-        for (int c = lane; c < p.chunks; c += 32) m = fmaxf(m, p.stats[int64_t(c) * p.T + row].x);
+        for (int c = lane; c < p.chunks; c += 32) m = fmaxf(m, stats[c].x);
         m = ib::warp_max(m);
         Stats st{m, 0.0f, 0.0f};
         for (int c = lane; c < p.chunks; c += 32) {
-            const float4 f = p.stats[int64_t(c) * p.T + row];
-            Stats o{f.x, f.y, f.z};
+            Stats o{stats[c].x, stats[c].y, stats[c].z};
             o.raise(m);
             st.s += o.s;
             st.d += o.d;
@@ -402,51 +428,43 @@ join_chunks_kernel(const JoinParams p) {
         st.d = ib::warp_sum(st.d);
         if (lane == 0) {
             total = st;
-            const int token = p.tokens ? p.tokens[row] : -1;
-            const float at = token >= 0 && token < p.V ? p.at[row] : 0.0f;
             ib::score::finish(st, token, at, p.scale, p.cap, p.V, p.logprob + row, p.entropy + row, p.status);
         }
     }
     if (p.top == 0) return;
-    auto list = [&](int c) { return p.lists + (int64_t(c) * p.T + row) * p.n; };
-    for (int c = threadIdx.x; c < p.chunks; c += JOIN_THREADS) heads[c] = list(c)[0];
-    __syncthreads();
     if (p.chunks >= p.top) {
         for (int c = threadIdx.x; c < p.chunks; c += JOIN_THREADS) {
             const unsigned long long k = heads[c];
-            int above = 0;
-            for (int j = 0; j < p.chunks; j++) above += heads[j] > k;
-            if (k != 0 && above == p.top - 1) bound = k;
+            if (k != 0 && beaten_by(heads, p.chunks, k) == p.top - 1) bound = k;
         }
-    } else {
-        unsigned long long most = 1;
-        for (int c = lane; c < p.chunks; c += 32) {
-            const unsigned long long k = list(c)[p.top - 1];
-            most = k > most ? k : most;
-        }
+    } else if (warp == 0) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const unsigned long long k = __shfl_xor_sync(0xffffffffu, most, o);
-            most = k > most ? k : most;
-        }
-        if (threadIdx.x == 0) bound = most;
+        for (int o = 16; o > 0; o >>= 1) lasts = max(lasts, __shfl_xor_sync(0xffffffffu, lasts, o));
+        if (lane == 0) bound = lasts;
     }
     __syncthreads();
-    unsigned long long* found = heads + p.chunks;
     const unsigned long long least = bound;
-    for (int i = threadIdx.x; i < p.chunks * p.top; i += JOIN_THREADS) {
-        const int c = i / p.top;
-        if (heads[c] < least) continue;
-        const unsigned long long k = list(c)[i - c * p.top];
-        if (k >= least) found[atomicAdd(&n_found, 1)] = k;
+    // (at most `top` lists: where there are more, as many as have a first key that reaches the top-th of them)
+    for (int c = threadIdx.x; c < p.chunks; c += JOIN_THREADS)
+        if (heads[c] >= least) chosen[atomicAdd(&n_chosen, 1)] = c;
+    __syncthreads();
+    const int n_keys = n_chosen * p.top;
+    constexpr int EACH = (MAX_TOP * MAX_TOP + JOIN_THREADS - 1) / JOIN_THREADS;
+    unsigned long long key[EACH];                                       // (requested together, looked at afterwards)
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        const int i = threadIdx.x + e * JOIN_THREADS, c = i / p.top;
+        key[e] = i < n_keys ? list(chosen[c])[i - c * p.top] : 0;
     }
+#pragma unroll
+    for (int e = 0; e < EACH; e++)
+        if (key[e] >= least) found[atomicAdd(&n_found, 1)] = key[e];
     __syncthreads();
     const int n = n_found;
     const Stats st = total;
     for (int i = threadIdx.x; i < n; i += JOIN_THREADS) {
         const unsigned long long k = found[i];
-        int above = 0;
-        for (int j = 0; j < n; j++) above += found[j] > k;
+        const int above = beaten_by(found, n, k);
         if (above < p.top) {
             p.top_ids[row * p.top + above] = int(ib::score::key_id(k));
             p.top_logprobs[row * p.top + above] = ib::score::logprob_of(st, ib::score::key_value(k), p.scale, p.cap);
@@ -538,10 +556,11 @@ IB_EXPORT int ib_head_logprobs_scratch(int64_t T, int64_t V, int64_t H, int top,
 }
 
 // x [T, H], w [V, H] bfloat16, 16-byte aligned; tokens int [T] or null; results as of ib_token_logprobs; scratch: ib_head_logprobs_scratch
-// bytes, 16-byte aligned, this call's own until it has run.
+// bytes, 16-byte aligned, this call's own until it has run; status: raised where a wait runs out; token_status (or null): set to 1 by a token
+// outside the vocabulary other than -1.
 IB_EXPORT int ib_head_logprobs(const void* x, const void* w, int64_t T, int64_t V, int64_t H, const int* tokens, int top, float scale, float cap,
                                float* logprob, float* entropy, int* top_ids, float* top_logprobs, void* scratch, int sm_count, int* status,
-                               cudaStream_t stream) {
+                               int* token_status, cudaStream_t stream) {
     if (T == 0) return IB_OK;
     int64_t bytes = 0;
     if (const int rc = ib_head_logprobs_scratch(T, V, H, top, sm_count, &bytes)) return rc;
@@ -555,22 +574,24 @@ IB_EXPORT int ib_head_logprobs(const void* x, const void* w, int64_t T, int64_t 
     p.n_kb = int((H + BK - 1) / BK);
     p.width = plan.width; p.tiles_n = plan.tiles; p.chunks = plan.chunks; p.row_blocks = plan.row_blocks;
     p.weights_once = plan.row_blocks == 1;
+    const int64_t ctas = int64_t(plan.row_blocks) * plan.group;
+    p.a_rows = int(((T + ctas - 1) / ctas + 7) / 8 * 8);
     p.scale = scale; p.cap = cap; p.tokens = tokens; p.status = status;
     char* s = static_cast<char*>(scratch);
     p.stats = reinterpret_cast<float4*>(s); s += int64_t(plan.chunks) * T * 16;
     p.lists = reinterpret_cast<unsigned long long*>(s); s += int64_t(plan.chunks) * T * 8 * n;
     p.at = reinterpret_cast<float*>(s);
     CUtensorMap ma, mb;
-    int rc = ib::get_map(x, T, H, BM, &ma);
+    int rc = ib::get_map(x, T, H, p.a_rows, &ma);
     if (rc) return rc;
     rc = ib::get_map(w, V, H, plan.width / plan.group, &mb);
     if (rc) return rc;
     if (plan.group == 1) rc = n == 0 ? launch_head<1, 0>(ma, mb, p, sm_count, stream) : n == 8 ? launch_head<1, 8>(ma, mb, p, sm_count, stream) : launch_head<1, MAX_TOP>(ma, mb, p, sm_count, stream);
     else rc = n == 0 ? launch_head<2, 0>(ma, mb, p, sm_count, stream) : n == 8 ? launch_head<2, 8>(ma, mb, p, sm_count, stream) : launch_head<2, MAX_TOP>(ma, mb, p, sm_count, stream);
     if (rc) return rc;
-    const JoinParams j{T, V, plan.chunks, n, top, scale, cap, tokens, p.stats, p.lists, p.at, logprob, entropy, top_ids, top_logprobs, status};
+    const JoinParams j{T, V, plan.chunks, n, top, scale, cap, tokens, p.stats, p.lists, p.at, logprob, entropy, top_ids, top_logprobs, token_status};
     const int lists = plan.chunks < top ? plan.chunks : top;           // lists that may hold a survivor, at most
-    const size_t smem = top ? size_t(plan.chunks + lists * top) * 8 : 0;
+    const size_t smem = size_t(plan.chunks) * 24 + size_t(lists) * top * 8;
     if (smem > 48 * 1024) return ib::fail(IB_ERR_ARG, "head_logprobs: %d chunks of the vocabulary are more than their join takes", plan.chunks);
     return ib::launch("join_chunks", join_chunks_kernel, dim3(unsigned(T)), dim3(JOIN_THREADS), smem, stream, 1u, j);
 }

@@ -397,7 +397,7 @@ def sm_count(device: torch.device) -> int:
 def head_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: int = 0, scale: float = 1.0,
                   softcap: float = 0.0, status: Optional[torch.Tensor] = None) -> TokenLogprobs:
     """``token_logprobs`` of the logits x @ w.T (x [T, H], w [V, H], both bfloat16 or both float32; scaled and capped as there), which are
-    not kept: bfloat16 rows go through a kernel that holds them in tensor memory only; up to 16 rows, rows that do not keep to 16 bytes and
+    not kept: bfloat16 rows go through a kernel that holds them in tensor memory only; up to 8 rows, rows that do not keep to 16 bytes and
     float32 go through logits of a few rows at a time. ``w`` is a loaded weight (as for ``linear``). A kernel whose bounded wait runs out
     says so in the device's status word."""
     if not (0 <= top <= 20 and 0 < scale < math.inf and 0 <= softcap < math.inf):

@@ -163,6 +163,19 @@ def test_tokens_outside_the_vocabulary_and_the_status_word():
     ops.token_logprobs(l, t.clamp(-1, 299), 2, status)
     assert status.item() == 0
     assert ops.token_logprobs(l[:0], t[:0], 3).top_ids.shape == (0, 3)
+    from infer_b200 import fast_ops
+    device_status = fast_ops.device_state(DEV).status
+    device_status.zero_()
+    for T in (4, 40, 300):
+        x, w, _ = _head(T, 64, 300, 1)
+        th = torch.full((T,), 299, dtype=torch.int32, device=DEV)
+        th[1], th[2] = 300, -7
+        status.zero_()
+        r = ops.head_logprobs(x, w, th, 2, status=status)
+        assert status.item() == 1 and r.logprob[1:3].isnan().all() and r.logprob[0].isfinite()
+        ops.head_logprobs(x, w, th, 2)
+    assert device_status.item() == 0, "a wrong token is the caller's: the device's word stays as it is"
+    assert ops.head_logprobs(x[:0], w, th[:0], 3).top_ids.shape == (0, 3)
 
 
 def test_calls_on_two_streams_and_in_a_graph_do_not_meet():
@@ -206,7 +219,7 @@ def _head(T, H, V, seed, dtype=torch.bfloat16):
     return x, w, t
 
 
-HEADS = [(1, 64, 300, 3), (16, 1536, 5000, 20), (17, 8, 1, 1), (17, 64, 5, 20), (33, 72, 130, 0), (64, 1536, 50257, 20), (100, 200, 301, 8), (128, 136, 1000, 9),
+HEADS = [(1, 64, 300, 3), (8, 1536, 5000, 20), (9, 64, 301, 20), (16, 1536, 5000, 20), (32, 1536, 9000, 5), (136, 72, 700, 5), (17, 8, 1, 1), (17, 64, 5, 20), (33, 72, 130, 0), (64, 1536, 50257, 20), (100, 200, 301, 8), (128, 136, 1000, 9),
          (129, 64, 300, 20), (130, 72, 5, 20), (256, 1536, 5003, 5), (257, 520, 1000, 0), (300, 1000, 32003, 20), (513, 128, 70000, 1), (1500, 96, 9001, 20),
          (77, 3584, 40000, 20)]
 
