@@ -314,12 +314,14 @@ class TokenLogprobs(NamedTuple):
 
 def _check_logprobs(rows: int, device, tokens: Optional[torch.Tensor], status: Optional[torch.Tensor]) -> None:
     for name, t, n in (("tokens", tokens, rows), ("status", status, 1)):
-        if t is None:
-            continue
-        if not t.is_cuda or t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        if t is not None:
             _check(t, name, torch.int32, (n,))
-        if t.device != device:
-            raise KernelError(f"{name} must lie on {device}, not on {t.device}")
+            if t.device != device:
+                raise KernelError(f"{name} must lie on {device}, not on {t.device}")
+
+
+def _plain_tokens(tokens: torch.Tensor, rows: int, device) -> bool:
+    return tokens.dtype is torch.int32 and tokens.device == device and tokens.shape == (rows,) and tokens.is_contiguous()
 
 
 def _refuse_distribution(top: int, scale: float, softcap: float) -> None:
@@ -339,10 +341,14 @@ def _logprobs_like(rows: int, top: int, device: torch.device):
 def _new_logprobs(rows: int, top: int, device: torch.device) -> TokenLogprobs:
     """(empty_like a kept tensor of the size, of one element expanded: 1.3 us a tensor where empty takes 2.3, four times a call.)"""
     a, ids, b = _logprobs_like(rows, top, device)
-    new, flat = torch.empty_like, torch.contiguous_format
-    return TokenLogprobs(new(a, memory_format=flat), new(a, memory_format=flat), new(ids, memory_format=flat), new(b, memory_format=flat))
+    new = torch.empty_like
+    return TokenLogprobs(new(a, memory_format=_FLAT), new(a, memory_format=_FLAT), new(ids, memory_format=_FLAT), new(b, memory_format=_FLAT))
 
 
+_FLAT = torch.contiguous_format
+
+
+@functools.lru_cache(maxsize=4096)
 def _logprobs_cluster(rows: int, vocab: int, sm_count: int) -> int:
     """CTAs that share a row of logits: as many as leave all rows running at once (two CTAs an SM; clusters of eight do not fit everywhere
     and get one), and each some 4,000 elements. (64 rows x 151,936, 20 alternatives, clusters of 8, 4, 2, 1: 41, 24, 29, 32 us.)"""
@@ -375,12 +381,14 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return token_logprobs(logits, tokens, top, status, scale, softcap, out)
-    _check_logprobs(T, device, tokens, status)
+    if status is not None or not (tokens is None or _plain_tokens(tokens, T, device)):
+        _check_logprobs(T, device, tokens, status)
     r = _new_logprobs(T, top, device) if out is None else out
     if T == 0:
         return r
-    _call(_token_logprobs_fn(), logits.data_ptr(), T, V, _ptr(tokens), top, scale, softcap, r.logprob.data_ptr(), r.entropy.data_ptr(),
-          r.top_ids.data_ptr(), r.top_logprobs.data_ptr(), _logprobs_cluster(T, V, sm_count(device)), _ptr(status), _stream())
+    a, b, c, d = r
+    _call(_token_logprobs_fn(), logits.data_ptr(), T, V, None if tokens is None else tokens.data_ptr(), top, scale, softcap, a.data_ptr(),
+          b.data_ptr(), c.data_ptr(), d.data_ptr(), _logprobs_cluster(T, V, sm_count(device)), _ptr(status), _stream())
     return r
 
 
@@ -407,7 +415,8 @@ def head_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[torch.Tenso
     if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return head_logprobs(x, w, tokens, top, scale, softcap, status)
-    _check_logprobs(T, device, tokens, status)
+    if status is not None or not (tokens is None or _plain_tokens(tokens, T, device)):
+        _check_logprobs(T, device, tokens, status)
     if T > 0 and x.dtype is torch.bfloat16:
         from . import fast_ops
         r = fast_ops.head_logprobs(x, w, tokens, top, scale, softcap, status)
@@ -459,11 +468,12 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else torch.float32 if residual is not None else x.dtype
     code = dtype_code(out_dtype)
-    for name, t, dtype, shape in (("bias", bias, torch.float32, (N,)), ("residual", residual, torch.float32, (M, N)), ("out", out, out_dtype, (M, N))):
-        if t is not None:
-            _check(t, name, dtype, shape)
-            if t.device != device:
-                raise KernelError(f"{name} must lie on {device}, not on {t.device}")
+    if bias is not None and not (bias.dtype is torch.float32 and bias.device == device and bias.shape == (N,) and bias.is_contiguous()):
+        _check_beside("bias", bias, torch.float32, (N,), device)
+    if residual is not None:
+        _check_beside("residual", residual, torch.float32, (M, N), device)
+    if out is not None:
+        _check_beside("out", out, out_dtype, (M, N), device)
     if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return linear_act(x, w, bias, activation, residual, out_dtype, out)
@@ -479,6 +489,12 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
     f = _fn("score", "ib_act_residual", _ACT_RESIDUAL_ARGS)
     _call(f, z.data_ptr(), _ptr(residual), out.data_ptr(), M * N, act, code, _stream())
     return out
+
+
+def _check_beside(name: str, t: torch.Tensor, dtype, shape, device) -> None:
+    _check(t, name, dtype, shape)
+    if t.device != device:
+        raise KernelError(f"{name} must lie on {device}, not on {t.device}")
 
 
 _ACT_RESIDUAL_ARGS = [c_void_p] * 3 + [c_int64, c_int, c_int, c_void_p]
