@@ -285,6 +285,7 @@ IB_EXPORT int ib_token_logprobs(const float* logits, int64_t rows, int64_t vocab
     if (vocab <= 0 || vocab >= (1LL << 30)) return ib::fail(IB_ERR_ARG, "token_logprobs: vocabulary %lld out of range", (long long)vocab);
     if (rows > 0x7fffffff / 8) return ib::fail(IB_ERR_ARG, "token_logprobs: too many rows (%lld)", (long long)rows);
     if (top < 0 || top > MAX_TOP) return ib::fail(IB_ERR_ARG, "token_logprobs: 0 to %d alternatives, not %d", MAX_TOP, top);
+    if (!logprob || !entropy || (top && (!top_ids || !top_logprobs))) return ib::fail(IB_ERR_ARG, "token_logprobs: results are needed");
     if (!(scale > 0.0f) || !(cap >= 0.0f)) return ib::fail(IB_ERR_ARG, "token_logprobs: the scale must be positive, the cap not negative");
     const Params p{logits, vocab, tokens, top, scale, cap, logprob, entropy, top_ids, top_logprobs, status};
     switch (cluster) {

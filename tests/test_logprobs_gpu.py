@@ -178,6 +178,43 @@ def test_tokens_outside_the_vocabulary_and_the_status_word():
     assert ops.head_logprobs(x[:0], w, th[:0], 3).top_ids.shape == (0, 3)
 
 
+def test_results_that_are_given():
+    from infer_b200 import ops
+    from infer_b200.ops import KernelError
+    l, t = _logits(5, 700, 1)
+    r = ops.TokenLogprobs(torch.empty(5, device=DEV), torch.empty(5, device=DEV), torch.empty(5, 3, dtype=torch.int32, device=DEV), torch.empty(5, 3, device=DEV))
+    assert ops.token_logprobs(l, t, 3, out=r) is r
+    check(r, l, l, t, 3)
+    for bad in (r._replace(entropy=r.entropy[:4]), r._replace(top_ids=r.top_ids.long()), r._replace(top_logprobs=r.top_logprobs.t()), r._replace(logprob=r.logprob.cpu())):
+        with pytest.raises(KernelError):
+            ops.token_logprobs(l, t, 3, out=bad)
+    for bad in (t.long(), t[:4], t.cpu(), t.expand(5, 5)[0].expand(2, 5)):
+        with pytest.raises(KernelError):
+            ops.token_logprobs(l, bad, 3)
+    with pytest.raises(KernelError):
+        ops.token_logprobs(l.half(), t, 3)
+    with pytest.raises(KernelError):
+        ops.token_logprobs(l.t(), None, 3)
+    with pytest.raises(KernelError):
+        ops.token_logprobs(l[:, :0], t, 3)
+
+
+def test_rows_beside_the_batch_are_left_as_they_are():
+    """Neither results behind the last row nor the inputs around a view are written; a batch inside a larger buffer."""
+    from infer_b200 import ops
+    big = torch.randn(9, 5003, device=DEV)
+    keep = big.clone()
+    l = big[2:7]
+    want = ops.token_logprobs(l.clone(), None, 4)
+    big[:2] = math.nan
+    big[7:] = math.nan
+    pads = [torch.full((12,), 7.0, device=DEV), torch.full((12,), 7.0, device=DEV), torch.full((12, 4), 7, dtype=torch.int32, device=DEV), torch.full((12, 4), 7.0, device=DEV)]
+    got = ops.token_logprobs(l, None, 4, out=ops.TokenLogprobs(*(p[3:8] for p in pads)))
+    for g, w, p in zip(got, want, pads):
+        assert torch.equal(g, w) and (p[:3] == 7).all() and (p[8:] == 7).all()
+    assert torch.equal(big[2:7], keep[2:7])
+
+
 def test_calls_on_two_streams_and_in_a_graph_do_not_meet():
     from infer_b200 import ops
     l, t = _logits(3, 151936, 5)

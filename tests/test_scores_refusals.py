@@ -8,7 +8,8 @@ from infer_b200.ops import KernelError
 
 @pytest.mark.parametrize("kw,what", [({"top": 21}, "alternatives"), ({"top": -1}, "alternatives"), ({"scale": 0.0}, "scale"), ({"scale": -1.0}, "scale"),
                                      ({"scale": float("nan")}, "scale"), ({"scale": float("inf")}, "scale"), ({"softcap": -1.0}, "cap"),
-                                     ({"softcap": float("inf")}, "cap"), ({"softcap": float("nan")}, "cap")])
+                                     ({"softcap": float("inf")}, "cap"), ({"softcap": float("nan")}, "cap"),
+                                     ({"scale": 1e39}, "scale"), ({"scale": 1e-20}, "scale"), ({"softcap": 1e-20}, "cap"), ({"softcap": 1e20}, "cap")])
 def test_distributions_that_are_none(kw, what):
     with pytest.raises(KernelError, match=what):
         ops.token_logprobs(torch.zeros(2, 5), None, **{"top": 0, **kw})
@@ -91,6 +92,8 @@ def test_scores_travel_through_a_scheduler_with_any_engine():
             if self.scored:
                 handle.scores = {b.rid: TokenScore(-1.5, 2.0, [(7, -1.5)]) for b in batch if b.sample is not None and b.sample.logprobs is not None}
             return handle
+    with pytest.raises(ValueError):
+        Scheduler(Fake(True)).submit(Request("c", [1], 2, 0, SampleParams(logprobs=21)))
     for overlap in (False, True):
         for scored in (False, True):
             sch = Scheduler(Fake(scored), SchedulerConfig(overlap=overlap))
