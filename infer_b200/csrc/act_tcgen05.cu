@@ -518,9 +518,9 @@ template <typename TOut> int launch_any(int slices, bool sums, const CUtensorMap
 }  // namespace
 
 // Width of a tile (32 .. 256, a multiple of 32) and slices of K (1, 2 or 4) for a product; sms: of the device. Cycles that a launch takes: rounds x
-// (k-blocks of a slice x (361 + 1.1 width) + what follows the last MMA), with that for a whole tile's epilogue 2,000 + 8 width, for
+// (k-blocks of a slice x (361 + 1.1 width) + what follows the last MMA), with that for a whole tile's epilogue 1,000 + 30 width, for
 // slices 13,000 beside their own columns' (two barriers, the push, another start).
-IB_EXPORT int ib_linear_act_plan(int64_t M, int64_t N, int64_t K, int sms, int* width, int* slices) {
+IB_EXPORT int ib_linear_act_plan(int64_t M, int64_t N, int64_t K, int sms, int* width, int* slices, int64_t* cycles) {
     if (M <= 0 || N <= 0 || K <= 0 || K % 8) return ib::fail(IB_ERR_ARG, "linear_act: sizes must be positive, K a multiple of 8");
     if (M >= (1LL << 30) || N >= (1LL << 30) || K >= (1LL << 30)) return ib::fail(IB_ERR_ARG, "linear_act: a size exceeds 2^30");
     const int64_t tm = (M + 2 * BM - 1) / (2 * BM), kb = (K + BK - 1) / BK;
@@ -534,12 +534,13 @@ IB_EXPORT int ib_linear_act_plan(int64_t M, int64_t N, int64_t K, int sms, int* 
             const int64_t tiles = tm * ((N + w - 1) / w);
             if (tiles >= (1LL << 28) || (s > 1 && tiles > 2 * room)) continue;
             const int64_t rounds = (tiles + room - 1) / room;
-            const int64_t cost = s == 1 ? rounds * kb * (361 + 11 * w / 10) + 2000 + 8 * w : rounds * ((kb + s - 1) / s * (361 + 11 * w / 10) + 13000 + 8 * w / s);
+            const int64_t cost = s == 1 ? rounds * kb * (361 + 11 * w / 10) + 1000 + 30 * w : rounds * ((kb + s - 1) / s * (361 + 11 * w / 10) + 13000 + 8 * w / s);
             if (least < 0 || cost < least) { least = cost; *width = w; *slices = s; }
         }
     }
     // (as many tiles, but no wider than they need to be)
     const int64_t tn = (N + *width - 1) / *width;
+    if (cycles) *cycles = least;
     if (least >= 0) *width = int(((N + tn - 1) / tn + 31) / 32 * 32);
     return least < 0 ? ib::fail(IB_ERR_ARG, "linear_act: too many tiles") : IB_OK;
 }

@@ -310,16 +310,31 @@ _ACT = {"IB_ACT": 1}              # the libraries whose kernels put an activatio
 
 
 @functools.lru_cache(maxsize=4096)
-def _act_plan(M: int, N: int, K: int, sm_count: int):
-    """What a product with an activation runs as: (True, tile width, slices of K) on pairs of SMs, (False, columns of a tile, slices of K) for
-    up to 128 rows, whose slices meet in a cluster's shared memory (neither needs scratch: calls may run on any streams at once);
-    None if the sizes are refused."""
-    if M <= 128:
-        plan = gemm_plan(M, N, K, sm_count)
-        return None if plan is None else (False, plan[1], plan[2])
-    width, slices = c_int(), c_int()
-    f = _fn("act_tc", "ib_linear_act_plan", [c_int64] * 3 + [c_int] + [c_void_p] * 2)
-    return (True, width.value, slices.value) if f(M, N, K, sm_count, ctypes.byref(width), ctypes.byref(slices)) == 0 else None
+def _act_plan(M: int, N: int, K: int, sm_count: int, float_out: bool = False):
+    """What a product with an activation runs as: (True, tile width, slices of K) on pairs of SMs, or up to 128 rows (False, columns of a tile,
+    slices of K) with the weights on the tensor core's rows; neither needs scratch: calls may run on any streams at once. None if the sizes
+    are refused.
+
+    Up to 128 rows two estimates in us decide: pairs the planner's cycles x 1.25 and 2.2; the others 3 + 0.33 for each k-block of a CTA (twice that
+    where the slices are no power of two: such clusters fit badly) + 0.1 for each column that a CTA finishes. Measured (others, pairs): 48 rows, 300 x 520
+    8.4 and 5.4, 1000 x 1000 5.6 and 6.7, 17920 x 1536 15.8 and 19.2; 96 rows, 8960 x 1536 16.4 and 13.1, 15000 x 5000 48.8 and 39.4,
+    1536 x 8960 13.9 and 18.0; 17 rows, 3584 x 18944 44.6 and 36.1. Float results of more than 1,536 elements of K in a chain (an error of 1.6e-6)
+    go to pairs, which sum in chains of 768 (17 rows, 18944 x 3584 24.5 and 35.8; the error 3.6e-6 and 0.7e-6)."""
+    width, slices, cycles = c_int(), c_int(), c_int64()
+    f = _fn("act_tc", "ib_linear_act_plan", [c_int64] * 3 + [c_int] + [c_void_p] * 3)
+    if f(M, N, K, sm_count, ctypes.byref(width), ctypes.byref(slices), ctypes.byref(cycles)) != 0:
+        return None
+    pairs = (True, width.value, slices.value)
+    other = gemm_plan(M, N, K, sm_count) if M <= 128 else None
+    if other is None:
+        return pairs
+    _, columns, cut = other[:3]
+    blocks = -(-K // 64)
+    chain = -(-blocks // cut)
+    if float_out and 64 * chain > 1536:
+        return pairs
+    others_us = 3 + 0.33 * chain * (1 if cut & (cut - 1) == 0 else 2) + 0.1 * -(-columns // cut)
+    return pairs if cycles.value / 1520 + 2.2 < others_us else (False, columns, cut)
 
 
 def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], act: int, residual: Optional[torch.Tensor],
@@ -342,7 +357,7 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], a
     if M <= 16:
         _call(_act_fn("gemvb"), *same, code, act, st.sm_count, st.status.data_ptr(), _stream())
         return True
-    plan = _act_plan(M, N, K, st.sm_count)
+    plan = _act_plan(M, N, K, st.sm_count, code == 0)
     if plan is None:
         return False
     pairs, width, slices = plan

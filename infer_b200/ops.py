@@ -368,7 +368,8 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     [0, V): NaN, and the status word (if given) is set to 1. ``scale`` / ``softcap``: the distribution is that of
     softcap * tanh(logits * scale / softcap) (-inf stays -inf), or logits * scale without a cap; alternatives go by ``logits``. ``out``: contiguous
     tensors of the result's shapes to write into.
-    Each call may run on any stream; a captured one reads its inputs anew at each replay."""
+    Each call may run on any stream; a captured one reads its inputs anew at each replay. The same call gives the same bits; a row's last bits
+    may differ where it lies otherwise to 16 bytes or among another number of rows."""
     if not (0 <= top <= 20 and 1e-18 <= scale <= 1e18 and (softcap == 0 or 1e-18 <= softcap <= 1e18)):
         _refuse_distribution(top, scale, softcap)
     if not logits.is_cuda or logits.dtype is not torch.float32 or not logits.is_contiguous():

@@ -46,7 +46,7 @@ def test_entry_points_refuse_sizes_they_do_not_take():
     act = load_module("act_tc")
     w, s = ctypes.c_int(), ctypes.c_int()
     for sizes in ((0, 5, 8), (4, 0, 8), (4, 5, 12), (1 << 30, 5, 8)):
-        assert act.ib_linear_act_plan(*map(i64, sizes), 148, ctypes.byref(w), ctypes.byref(s)) < 0 and act.ib_last_error()
+        assert act.ib_linear_act_plan(*map(i64, sizes), 148, ctypes.byref(w), ctypes.byref(s), None) < 0 and act.ib_last_error()
     null = ctypes.c_void_p()
     for args in ((12, 1, 0, 64, 1), (64, 1, 9, 64, 1), (64, 1, 0, 48, 1), (64, 1, 0, 64, 3), (64, 7, 0, 64, 1), (64, 1, 0, 64, 4)):
         K, dtype, a, width, slices = args
@@ -61,6 +61,19 @@ def test_plans_of_products_stay_within_the_kernels_ranges(M, N, K):
         pairs, width, slices = fast_ops._act_plan(M, N, K, sms)
         assert pairs and width % 32 == 0 and 32 <= width <= 256 and slices in (1, 2, 4)
         assert slices == 1 or -(-K // 64) >= 2 * slices
+
+
+@pytest.mark.parametrize("M", [17, 40, 100, 128])
+@pytest.mark.parametrize("N,K", [(33, 64), (300, 520), (1536, 8960), (18944, 3584), (18944, 18944), (40, 18944)])
+def test_plans_of_few_rows(M, N, K):
+    from infer_b200 import fast_ops
+    for float_out in (False, True):
+        pairs, width, slices = fast_ops._act_plan(M, N, K, 148, float_out)
+        if pairs:
+            assert width % 32 == 0 and 32 <= width <= 256 and slices in (1, 2, 4)
+        else:
+            assert width in (16, 32, 64, 128) and 1 <= slices <= 8
+            assert not float_out or -(-(-(-K // 64)) // slices) * 64 <= 1536, "a long chain of float sums"
 
 
 @pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 151936), (18, 151936), (19, 151936), (74, 151936), (75, 50257), (149, 151936), (5000, 300)])
