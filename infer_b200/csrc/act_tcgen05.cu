@@ -1,5 +1,5 @@
-// out = residual + act(x . w^T + bias) on pairs of SMs, for more than 128 rows: x [M, K], w [N, K] bfloat16, bias and residual float, out float or
-// bfloat16, rounded once.
+// out = residual + act(x . w^T + bias) on pairs of SMs, for more than 128 rows and for fewer where that is faster: x [M, K], w [N, K] bfloat16, bias
+// and residual float, out float or bfloat16, rounded once.
 //
 // Two CTAs (a pair) form 256 rows x W columns with tcgen05.mma.cta_group::2: each loads its 128 rows of x and half of the W rows of w by TMA
 // into a ring of stages of two k-blocks (64 elements each), the first CTA's MMA warp issues for both, and each keeps the sums of its
@@ -15,7 +15,9 @@
 // distributed shared memory, into what was the operand ring, and the owners add the slices in ascending order. No scratch in global memory, no
 // counters, nothing that two calls could share.
 //
-// Bound by the MMAs, or by the way from L2: a k-block of a pair takes 361 + 1.1 W cycles (measured; the MMAs alone 2 W).
+// Bound by the MMAs, or by the way from L2: a k-block of a pair takes 361 + 1.1 W cycles (measured; the MMAs alone 2 W). us in a graph, gelu_tanh,
+// bfloat16 and float results: 2048 x 18944 x 3584 180 (1,545 TFLOP/s) and 237, 2048 x 8960 x 1536 47 and 62, 500 x 1536 x 8960 in four slices 23 and 23,
+// 1000 x 1536 x 1536 12.1 and 14.9.
 #include "common.cuh"
 #include "score.cuh"
 #include "tc_ops.cuh"
