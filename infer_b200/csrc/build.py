@@ -44,6 +44,7 @@ MODULES: Dict[str, str] = {
     "latent_pf": "latent_prefill.cu",   # the same attention for prompt portions: per-head keys and values, tensor cores
     "score": "score_ops.cu",     # log probabilities, entropies and alternatives from logits; activations behind a product
     "score_head": "score_head.cu",      # the same from the rows in front of a head, the logits in tensor memory only
+    "lin32_cut": "linear_f32_cut.cu",   # 32-bit products with an activation for batches of rows, the operands cut into thirds beforehand
     "act_tc": "act_tcgen05.cu",  # products with an activation between bias and residual, on pairs of SMs
     "gemvb": "gemv_bulk.cu",
     "gemm": "gemm_tcgen05.cu",
@@ -51,7 +52,7 @@ MODULES: Dict[str, str] = {
     "attn_tc": "attention_tc.cu",
     "capi": "capi.cpp",          # host code only: the C handle API over the engine (needs the interpreter's headers)
 }
-HEADERS = ["common.cuh", "gemm_static.h", "per_device.h", "score.cuh", "tc_ops.cuh", "tma_map.cuh"]
+HEADERS = ["act_end.cuh", "common.cuh", "gemm_static.h", "per_device.h", "score.cuh", "tc_ops.cuh", "tma_map.cuh"]
 # modules that are compiled per model size: the variant that build_all() makes (others are built at first use)
 DEFAULT_DEFINES = {"attn": {"IB_HEAD_DIM": 128}, "attn_tc": {"IB_HEAD_DIM": 128}, "latent_pf": {"IB_QK_DIM": 128, "IB_V_DIM": 128},
                    "talk_pf": {"IB_HEAD_DIM": 128, "IB_V_DIM": 128, "IB_HEADS": 12}}

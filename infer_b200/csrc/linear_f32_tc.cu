@@ -485,7 +485,7 @@ linear32_tc_kernel(const Params p) {
     }
 }
 
-struct Plan { int nt, groups, share; };
+struct Plan { int nt, groups, share; int64_t blocks; };      // blocks: what the chosen share costs, below
 
 // Groups: as many as give the tiles of features alone work for every SM, a power of two, at most 8, of at least two blocks each. From N, K
 // and the device alone, never from M: the order of a row's sums must not depend on how many rows there are.
@@ -517,7 +517,7 @@ Plan make_plan(int64_t M, int64_t N, int64_t K, int sms) {
         const int64_t at_once = z == 1 ? sms : (z == 2 ? sms - 4 : (sms - sms / 7) / z * z);
         const int64_t rounds = (tiles * z + at_once - 1) / at_once;
         const int64_t cost = rounds * ((blocks + z - 1) / z + 4 + (z > 1 ? 2 : 0));
-        if (best == 0 || cost < best) { best = cost; q.share = z; }
+        if (best == 0 || cost < best) { best = q.blocks = cost; q.share = z; }
     }
     return q;
 }
@@ -549,6 +549,14 @@ IB_EXPORT int ib_linear_f32_tc_takes(int64_t N, int64_t K) {
     return N >= 1024 && K >= 1024 && N <= 65535LL * BM && K < (1LL << 31) ? 1 : 0;
 #endif
 }
+
+#ifdef IB_ACT
+// Estimated ns: 1,200 for each block of the plan's count and 8,000. (512 x 17920 x 1536 277,000, measured 285; 301 x 2301 x 1000 32,000 and 39;
+// 512 x 1536 x 8960 181,000 and 172; 400 x 500 x 500 18,000 and 12.)
+IB_EXPORT int64_t ib_linear_f32_tc_ns(int64_t M, int64_t N, int64_t K, int sm_count) {
+    return M <= 0 || N <= 0 ? 0 : 8000 + 1200 * make_plan(M, N, K, sm_count).blocks;
+}
+#endif
 
 // residual may be out. w_ready: as in ib_linear_f32.
 IB_EXPORT int ib_linear_f32_tc(const float* x, const float* w, const float* bias, const float* residual, float* out, int64_t M, int64_t N,

@@ -610,6 +610,9 @@ class Engine:
                     141: "a copy wait of the head's log probabilities ran out", 142: "an operand wait of the head's log probabilities ran out",
                     143: "an accumulator wait of the head's log probabilities ran out", 151: "a copy wait of a product with an activation ran out",
                     152: "an operand wait of a product with an activation ran out", 153: "an accumulator wait of a product with an activation ran out",
+                    161: "a copy wait of a 32-bit product with an activation ran out",
+                    162: "an operand wait of a 32-bit product with an activation ran out",
+                    163: "an accumulator wait of a 32-bit product with an activation ran out",
                     108: "the prefill attention's shared memory does not start on a 1024-byte boundary",
                     }.get(code, f"code {code}")
             raise RuntimeError(f"device status word was raised: {what}")

@@ -348,7 +348,12 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], a
         if code != 0:
             return False
         if _f32_act_on_tensor_cores(M, N, K):
-            _call(_act_fn("lin32_tc"), *same, st.sm_count, 1, act, st.status.data_ptr(), _stream())
+            cut = _f32_cut_plan(M, N, K, st.sm_count)
+            if cut is None:
+                _call(_act_fn("lin32_tc"), *same, st.sm_count, 1, act, st.status.data_ptr(), _stream())
+            else:
+                scratch = x.new_empty((cut[1],), dtype=torch.uint8)
+                _call(_act_fn("lin32_cut"), *same, act, cut[0], scratch.data_ptr(), st.sm_count, st.status.data_ptr(), _stream())
         else:
             _call(_act_fn("lin32"), *same, 0, st.sm_count, 1, act, _stream())
         return True
@@ -372,8 +377,8 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], a
 def _act_fn(module: str):
     name, args = {"lin32_tc": ("ib_linear_f32_tc", [c_int] * 3 + [c_void_p] * 2), "lin32": ("ib_linear_f32", [c_int] * 4 + [c_void_p]),
                   "gemvb": ("ib_linear_skinny_act", [c_int] * 3 + [c_void_p] * 2), "gemm": ("ib_gemm_tc", [c_int] * 5 + [c_void_p] * 4),
-                  "act_tc": ("ib_linear_act", [c_int] * 5 + [c_void_p] * 2)}[module]
-    return _fn(module, name, [c_void_p] * 5 + [c_int64] * 3 + args, None if module in ("gemvb", "act_tc") else _ACT)
+                  "lin32_cut": ("ib_linear_f32_cut", [c_int] * 2 + [c_void_p, c_int] + [c_void_p] * 2), "act_tc": ("ib_linear_act", [c_int] * 5 + [c_void_p] * 2)}[module]
+    return _fn(module, name, [c_void_p] * 5 + [c_int64] * 3 + args, None if module in ("gemvb", "act_tc", "lin32_cut") else _ACT)
 
 
 def _f32_act_on_tensor_cores(M: int, N: int, K: int) -> bool:
@@ -382,6 +387,23 @@ def _f32_act_on_tensor_cores(M: int, N: int, K: int) -> bool:
     301 x 1000 x 200 11.1 and 15.9, 1000 x 500 x 500 25.5 and 14.6, 2000 x 1000 x 128 29.8 and 24.6, 8 x 16000 x 400 17.3 and 11.4,
     333 x 32003 x 1000 643 and 294. (Not by N and K alone as the engine's products: a row's bits may depend on how many rows there are.)"""
     return N >= 128 and K >= 128 and M >= 2 and M * N * K >= 30_000_000
+
+
+@functools.lru_cache(maxsize=4096)
+def _f32_cut_plan(M: int, N: int, K: int, sm_count: int) -> Optional[tuple]:
+    """(Tile width, bytes of scratch) where a product of floats on the tensor cores cuts its operands into bfloat16 numbers beforehand; None where it
+    cuts them on its way, which takes less by the two kernels' estimates: measured (beforehand, on its way; us) 301 x 2301 x 1000 29 and 39,
+    333 x 32003 x 1000 207 and 297, 2000 x 4000 x 2000 172 and 338, 512 x 1536 x 8960 144 and 172, 129 x 8960 x 1536 61 and 66; but 128 x 8960 x 1536
+    61 and 43, 129 x 1000 x 1000 25 and 18, 256 x 1536 x 8960 133 and 107."""
+    width, nbytes, ns = c_int(), c_int64(), c_int64()
+    f = _fn("lin32_cut", "ib_linear_f32_cut_plan", [c_int64] * 3 + [c_int] + [c_void_p] * 3)
+    if f(M, N, K, sm_count, ctypes.byref(width), ctypes.byref(nbytes), ctypes.byref(ns)) != 0 or nbytes.value > F32_CUT_SCRATCH:
+        return None
+    other = _fn("lin32_tc", "ib_linear_f32_tc_ns", [c_int64] * 3 + [c_int], _ACT, c_int64)
+    return (width.value, nbytes.value) if ns.value < other(M, N, K, sm_count) else None
+
+
+F32_CUT_SCRATCH = 1 << 29      # bytes of scratch that such a product takes at most
 
 
 HEAD_STREAMED = 8              # rows up to which the streaming product reads the matrix faster than the tensor-core kernel does
@@ -398,7 +420,7 @@ def head_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[torch.Tenso
     if H % 8 or (px & 15) or (pw & 15):
         return None
     st = device_state(x.device)
-    r = ops._new_logprobs(T, top, x.device)
+    r = ops._new_logprobs(T, top, x)
     results = r.logprob.data_ptr(), r.entropy.data_ptr(), r.top_ids.data_ptr(), r.top_logprobs.data_ptr()
     asked = None if tokens is None else tokens.data_ptr()
     if T <= HEAD_STREAMED:

@@ -333,17 +333,9 @@ def _refuse_distribution(top: int, scale: float, softcap: float) -> None:
     raise KernelError(f"the logits' cap must lie between 1e-18 and 1e18, or be 0 for none, not {softcap}")
 
 
-@functools.lru_cache(maxsize=64)
-def _logprobs_like(rows: int, top: int):
-    meta = lambda shape, dtype: torch.empty(shape, dtype=dtype, device="meta")
-    return meta((rows,), torch.float32), meta((rows, top), torch.int32), meta((rows, top), torch.float32)
-
-
-def _new_logprobs(rows: int, top: int, device: torch.device) -> TokenLogprobs:
-    """(empty_like a tensor without memory: a microsecond less than empty, four times a call.)"""
-    a, ids, b = _logprobs_like(rows, top)
-    new = torch.empty_like
-    return TokenLogprobs(new(a, device=device), new(a, device=device), new(ids, device=device), new(b, device=device))
+def _new_logprobs(rows: int, top: int, beside: torch.Tensor) -> TokenLogprobs:
+    new, f32 = beside.new_empty, torch.float32
+    return TokenLogprobs(new((rows,), dtype=f32), new((rows,), dtype=f32), new((rows, top), dtype=torch.int32), new((rows, top), dtype=f32))
 
 
 @functools.lru_cache(maxsize=4096)
@@ -384,7 +376,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     if status is not None or not (tokens is None or _plain_tokens(tokens, T, device)):
         _check_logprobs(T, device, tokens, status)
     if out is None:
-        r = _new_logprobs(T, top, device)
+        r = _new_logprobs(T, top, logits)
     else:
         r = out
         for t, dtype, shape in zip(r, (torch.float32, torch.float32, torch.int32, torch.float32), ((T,), (T,), (T, top), (T, top))):
@@ -427,7 +419,7 @@ def head_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[torch.Tenso
         r = fast_ops.head_logprobs(x, w, tokens, top, scale, softcap, status)
         if r is not None:
             return r
-    r = _new_logprobs(T, top, device)
+    r = _new_logprobs(T, top, x)
     step = max(1, min(T, HEAD_LOGITS // V))
     logits = x.new_empty((step, V), dtype=torch.float32)
     for lo in range(0, T, step):

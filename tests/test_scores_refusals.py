@@ -52,6 +52,18 @@ def test_entry_points_refuse_sizes_they_do_not_take():
         K, dtype, a, width, slices = args
         rc = act.ib_linear_act(null, null, null, null, null, i64(4), i64(5), i64(K), dtype, a, width, slices, 148, null, null)
         assert rc < 0 and act.ib_last_error(), args
+    cut = load_module("lin32_cut")
+    ns = ctypes.c_int64()
+    for sizes in ((0, 5, 8), (4, 0, 8), (4, 5, 0), (4, 5, 16385), (1 << 30, 5, 8), (4, 1 << 30, 8)):
+        assert cut.ib_linear_f32_cut_plan(*map(i64, sizes), 148, ctypes.byref(w), ctypes.byref(n), ctypes.byref(ns)) < 0 and cut.ib_last_error()
+    assert cut.ib_linear_f32_cut_plan(i64(4), i64(5), i64(8), 1, ctypes.byref(w), ctypes.byref(n), ctypes.byref(ns)) < 0
+    for sizes in ((1, 1, 1), (301, 2301, 1001), (5000, 130, 16384)):
+        assert cut.ib_linear_f32_cut_plan(*map(i64, sizes), 148, ctypes.byref(w), ctypes.byref(n), ctypes.byref(ns)) == 0
+        assert w.value in (32, 64, 96, 128) and n.value == 6 * (sizes[0] + sizes[1]) * -(-sizes[2] // 8) * 8
+    some = ctypes.c_void_p(64)
+    for K, a, width, scratch, status in ((16385, 0, 64, some, some), (64, 9, 64, some, some), (64, -1, 64, some, some), (64, 0, 48, some, some),
+                                         (64, 0, 64, null, some), (64, 0, 64, ctypes.c_void_p(8), some), (64, 0, 64, some, null)):
+        assert cut.ib_linear_f32_cut(null, null, null, null, null, i64(4), i64(5), i64(K), a, width, scratch, 148, status, null) < 0 and cut.ib_last_error()
 
 
 @pytest.mark.parametrize("M,N,K", [(129, 1, 8), (129, 18944, 64), (300, 1000, 1536), (500, 1536, 8960), (2048, 18944, 3584), (4096, 33, 18944), (1 << 20, 7, 8)])
