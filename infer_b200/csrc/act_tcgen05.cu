@@ -16,7 +16,7 @@
 // counters, nothing that two calls could share.
 //
 // Bound by the MMAs, or by the way from L2: a k-block of a pair takes 361 + 1.1 W cycles (measured; the MMAs alone 2 W). us in a graph, gelu_tanh,
-// bfloat16 and float results: 2048 x 18944 x 3584 180 (1,545 TFLOP/s) and 237, 2048 x 8960 x 1536 47 and 62, 500 x 1536 x 8960 in four slices 23 and 23,
+// bfloat16 and float results: 2048 x 18944 x 3584 180 (1,545 TFLOP/s) and 237, 2048 x 8960 x 1536 47 and 62, 500 x 1536 x 8960 in four slices 22 and 22,
 // 1000 x 1536 x 1536 12.1 and 14.9.
 #include "act_end.cuh"
 #include "tma_map.cuh"
@@ -231,7 +231,7 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
         __syncwarp();
     }
     if constexpr (S > 1) {
-        cluster_sync();                                  // every MMA of the cluster is done: the rings are free
+        cluster_meet();                                  // every MMA of the cluster is done: the rings are free
         // [slice][group of four columns][row][4] of the columns that this CTA owns: width / S from width / S * slice on (32 bytes behind each
         // group: lanes that read two rows of four groups do not meet in a bank)
         const int own = p.width / S, quad = warp & 3, r = quad * 32 + lane, half = (warp - 2) >> 2, cols = p.width / 2;
@@ -298,7 +298,7 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     }
     tc_fence_before();
     __syncthreads();
-    cluster_sync();                                      // no CTA's shared memory is needed by another any more
+    cluster_meet();                                      // no CTA's shared memory is needed by another any more
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(uint32_t(TMEM_COLS)) : "memory");

@@ -317,7 +317,7 @@ cut_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     }
     tc_fence_before();
     __syncthreads();
-    cluster_sync();                                      // neither CTA's shared memory is needed by the other any more
+    cluster_meet();                                      // neither CTA's shared memory is needed by the other any more
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(uint32_t(TMEM_COLS)) : "memory");
