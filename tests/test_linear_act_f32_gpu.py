@@ -136,3 +136,11 @@ def test_calls_on_two_streams_and_in_a_graph_do_not_meet():
                 g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(c, fresh) for c in captured)
+
+
+def test_every_result_computed_again():
+    """All results infinite, the longest K: the warps that compute them again are not done before the issuer would wait, and are done in time."""
+    x = torch.full((300, 16384), math.inf, device=DEV)
+    w = torch.rand(260, 16384, device=DEV) + 0.5
+    y = _cut(x, w, None, "none", None, 128)
+    assert torch.equal(y, torch.full((300, 260), math.inf, device=DEV))
