@@ -28,13 +28,14 @@ template <int N> __device__ __forceinline__ float largest_of(const float (&z)[N]
 }
 
 // The logits of N sums under a cap, without tanhf's branches: for |u| <= 0.6 an odd polynomial (a minimax fit of tanh(u) / u in u^2, off by
-// 2.5e-9 before its roundings: 2 x 2^-24 of the result with them), else 1 - 2 / (1 + e^2|u|) (5 x 2^-24). A thread goes by the largest of its own.
-template <int N> __device__ __forceinline__ void cap_logits(float (&l)[N], const float (&z)[N], float scale, float cap) {
+// 2.5e-9 before its roundings: 2 x 2^-24 of the result with them), else 1 - 2 / (1 + e^2|u|) (5 x 2^-24). A thread goes by the largest of its own, one whose
+// results are not needed (`counts`) by the polynomial.
+template <int N> __device__ __forceinline__ void cap_logits(float (&l)[N], const float (&z)[N], float scale, float cap, bool counts = true) {
     const float to_u = scale / cap;
     float most = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; i++) { l[i] = z[i] * to_u; most = fmaxf(most, l[i] == -INFINITY ? 0.0f : fabsf(l[i])); }
-    if (most <= 0.6f) {
+    if (most <= 0.6f || !counts) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const float u = l[i], q = u * u;

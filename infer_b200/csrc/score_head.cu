@@ -126,9 +126,10 @@ template <int N> struct Best {
     }
     // Takes what it wants of 32 neighbouring columns, the largest first (z is used up). One branch for the warp and a round for as many columns as
     // a lane wants: with a branch for each column and lane a single warp on its scheduler waited for most of its time.
-    __device__ __forceinline__ void take(float (&z)[32], float top, int n0) {
+    // (`row`: whether the lane has a row; others hold whatever shared memory held, which would keep the warp.)
+    __device__ __forceinline__ void take(float (&z)[32], float top, int n0, bool row) {
         for (;; top = ib::score::largest_of<32>(z)) {
-            const bool mine = wants(top);
+            const bool mine = row && wants(top);
             if (!__any_sync(0xffffffffu, mine)) return;
             int at = 0;
 #pragma unroll
@@ -141,7 +142,7 @@ template <int N> struct Best {
 };
 template <> struct Best<0> {
     __device__ __forceinline__ void clear() {}
-    __device__ __forceinline__ void take(float (&)[32], float, int) {}
+    __device__ __forceinline__ void take(float (&)[32], float, int, bool) {}
 };
 
 struct HeadParams {
@@ -324,13 +325,13 @@ head_logprobs_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                         }
                         if (p.cap > 0.0f) {
                             float l[32];
-                            ib::score::cap_logits<32>(l, z, p.scale, p.cap);
-                            st.add<32>(l, ib::score::largest_of<32>(l));
-                            best.take(z, ib::score::largest_of<32>(z), n0);
+                            ib::score::cap_logits<32>(l, z, p.scale, p.cap, mine);
+                            st.add<32>(l, mine ? ib::score::largest_of<32>(l) : -INFINITY);
+                            best.take(z, ib::score::largest_of<32>(z), n0, mine);
                         } else {
                             const float top = ib::score::largest_of<32>(z);
-                            st.add<32>(z, top, p.scale);
-                            best.take(z, top, n0);
+                            st.add<32>(z, mine ? top : -INFINITY, p.scale);
+                            best.take(z, top, n0, mine);
                         }
                     }
                 }
