@@ -106,17 +106,22 @@ __device__ __forceinline__ float4 bias_of(const EndParams& p, int64_t n) {
     return f;
 }
 // v[4 i + j] = column j of number i with its bias. ACT < 0: which activation is a parameter of the launch.
-template <int ACT, typename TOut>
-__device__ __forceinline__ void finish_four(const EndParams& p, const Four& f, float (&v)[16], const float4 (&add)[4]) {
+template <int ACT>
+__device__ __forceinline__ void values_of(const EndParams& p, float (&v)[16], const float4 (&add)[4]) {
     if constexpr (ACT < 0) ib::score::activate_all<16>(v, p.act);
     else {
 #pragma unroll
         for (int i = 0; i < 16; i++) v[i] = ib::score::activate(v[i], ACT);
     }
 #pragma unroll
+    for (int i = 0; i < 4; i++) { v[4 * i] += add[i].x; v[4 * i + 1] += add[i].y; v[4 * i + 2] += add[i].z; v[4 * i + 3] += add[i].w; }
+}
+template <typename TOut>
+__device__ __forceinline__ void store_four(const EndParams& p, const Four& f, const float (&v)[16]) {
+#pragma unroll
     for (int i = 0; i < 4; i++) {
         if (!(f.live >> i & 1)) continue;
-        const float x = v[4 * i] + add[i].x, y = v[4 * i + 1] + add[i].y, z = v[4 * i + 2] + add[i].z, w = v[4 * i + 3] + add[i].w;
+        const float x = v[4 * i], y = v[4 * i + 1], z = v[4 * i + 2], w = v[4 * i + 3];
         TOut* at = static_cast<TOut*>(p.out) + f.at + i * f.step;
         if (p.vec) {
             if constexpr (sizeof(TOut) == 4) *reinterpret_cast<float4*>(at) = make_float4(x, y, z, w);
@@ -183,8 +188,36 @@ struct TileEnd {
         f.left -= 16;
         f.live = f.left > 0 ? rows : 0u;
         if (p.residual && more) residual_of(p, f, add);
-        finish_four<ACT, TOut>(p, here, x, now);
+        values_of<ACT>(p, x, now);
         __syncwarp();                                             // the block has been read
+        if (sizeof(TOut) == 4 || p.vec) store_four<TOut>(p, here, x);
+        else store_columns<TOut>(p, mem, here, x);
+    }
+    // Rows of 16-bit numbers that do not keep to four columns: the values go back into the block, and sixteen lanes store a row's columns, two rows at
+    // a time. (A lane's four columns one by one touch every sector four times: 2000 x 4001 x 512 35 us, this way 26, with 4,000 columns 14.
+    // Floats lose by it: 776 x 13581 x 264 on the 32-bit kernel 78 and 91.)
+    template <typename TOut>
+    __device__ __forceinline__ void store_columns(const EndParams& p, uint8_t* mem, const Four& here, const float (&x)[16]) {
+        const int lane = threadIdx.x & 31, unit = lane & 3, column = lane & 15;
+        uint32_t there = 0;                                       // bit r: row r of the warp is one
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            *reinterpret_cast<float4*>(mem + (8 * i + (lane >> 2)) * 64 + ((unit ^ (((8 * i + (lane >> 2)) >> 1) & 3)) << 4)) = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            const uint32_t four = __ballot_sync(0xffffffffu, rows >> i & 1);      // (a row's four lanes say the same)
+#pragma unroll
+            for (int r = 0; r < 8; r++) there |= (four >> (4 * r) & 1u) << (8 * i + r);
+        }
+        __syncwarp();
+        const bool inside = column < here.left + 4 * unit;
+        TOut* to = static_cast<TOut*>(p.out) + here.at - (lane >> 2) * p.N - 4 * unit + (lane >> 4) * p.N + column;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int row = 2 * i + (lane >> 4);
+            const float v = *reinterpret_cast<const float*>(mem + row * 64 + (((column >> 2) ^ ((row >> 1) & 3)) << 4) + (column & 3) * 4);
+            if (inside && (there >> row & 1)) to[0] = ib::from_f32<TOut>(v);
+            to += 2 * p.N;
+        }
+        __syncwarp();
     }
 };
 

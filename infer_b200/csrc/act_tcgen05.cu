@@ -291,7 +291,8 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                     }
                     v[4 * j] = z.x + bias[k & 1][j].x; v[4 * j + 1] = z.y + bias[k & 1][j].y; v[4 * j + 2] = z.z + bias[k & 1][j].z; v[4 * j + 3] = z.w + bias[k & 1][j].w;
                 }
-                finish_four<ACT, TOut>(p, f, v, add[k & 1]);
+                values_of<ACT>(p, v, add[k & 1]);
+                store_four<TOut>(p, f, v);
                 if (k + 2 < batches) request(k + 2, bias[k & 1], add[k & 1]);
             }
         }

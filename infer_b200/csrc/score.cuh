@@ -130,13 +130,37 @@ __device__ __forceinline__ float times_sigmoid2(float x, float y) {
     return x * r;
 }
 
+// z Phi(z), Phi the normal distribution. With s = |z|: Phi(-s) = e^(-s^2 / 2) t P(t), t = 1 / (1 + 0.26 s), P a fit to erfcx (least largest relative
+// error over 0 <= s <= 14.5: 2.8e-8); what s^2 and its product with log2(e) / 2 lose in rounding goes in by a factor. Off by 8 x 2^-24 of the
+// result from z = -6 on and by 22 x 2^-24 at -12.6 (measured against 64 bits). With erfcf in its place 776 x 13580 x 264 took
+// 53 us (37), in 32 bits 170 (109).
+__device__ __forceinline__ float gelu(float z) {
+    const float s = fminf(fabsf(z), 20.0f), h = s * s, y = h * -0.72134752f;
+    float off = fmaf(h, -0.72134752f, -y);
+    off = fmaf(fmaf(s, s, -h), -0.72134752f, off);
+    float t;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(s, 0.26f, 1.0f)));
+    float p = fmaf(t, 0.03023030050098896f, -0.15149444341659546f);
+    p = fmaf(t, p, 0.24873320758342743f);
+    p = fmaf(t, p, -0.1477893441915512f);
+    p = fmaf(t, p, 0.1587587594985962f);
+    p = fmaf(t, p, 0.05196481943130493f);
+    p = fmaf(t, p, 0.10278867930173874f);
+    p = fmaf(t, p, 0.10305097699165344f);
+    p = fmaf(t, p, 0.10375702381134033f);
+    float e = exp2_fast(y);
+    e = fmaf(e, off * 0.6931472f, e);
+    const float q = e * (t * p);
+    return z * (z >= 0.0f ? 1.0f - q : q);
+}
+
 __device__ __forceinline__ float activate(float z, int act) {
     switch (act) {
         case RELU: return z > 0.0f ? z : (z != z ? z : 0.0f);
         case RELU_SQUARED: { const float r = z > 0.0f ? z : (z != z ? z : 0.0f); return r * r; }
         // 0.5 z (1 + tanh u) = z sigmoid(2 u), u = sqrt(2/pi) (z + 0.044715 z^3); the constants are 2 sqrt(2/pi) log2(e) and 0.044715 of it
         case GELU_TANH: return times_sigmoid2(z, z * fmaf(z * z, 0.10294324f, 2.3022082f));
-        case GELU: return 0.5f * z * erfcf(-0.70710678118654752f * z);
+        case GELU: return gelu(z);
         case SILU: return times_sigmoid2(z, LOG2E * z);
     }
     return z;

@@ -318,8 +318,8 @@ def _act_plan(M: int, N: int, K: int, sm_count: int, float_out: bool = False):
     Up to 128 rows two estimates in us decide: pairs the planner's cycles x 1.25 and 2.2; the others 3 + 0.33 for each k-block of a CTA (twice that
     where the slices are no power of two: such clusters fit badly) + 0.1 for each column that a CTA finishes. Measured (others, pairs): 48 rows, 300 x 520
     8.4 and 5.4, 1000 x 1000 5.6 and 6.7, 17920 x 1536 15.8 and 19.2; 96 rows, 8960 x 1536 16.4 and 13.1, 15000 x 5000 48.8 and 39.4,
-    1536 x 8960 13.9 and 18.0; 17 rows, 3584 x 18944 44.6 and 36.1. Float results of more than 1,536 elements of K in a chain (an error of 1.6e-6)
-    go to pairs, which sum in chains of 768 (17 rows, 18944 x 3584 24.5 and 35.8; the error 3.6e-6 and 0.7e-6)."""
+    1536 x 8960 13.9 and 18.0; 17 rows, 3584 x 18944 44.6 and 36.1. Float results of more than 768 elements of K in a chain (an error of 1.3e-6
+    with 1,280) go to pairs, which sum in chains of 768 (17 rows, 18944 x 3584 24.5 and 35.8; the error 3.6e-6 and 0.7e-6)."""
     width, slices, cycles = c_int(), c_int(), c_int64()
     f = _fn("act_tc", "ib_linear_act_plan", [c_int64] * 3 + [c_int] + [c_void_p] * 3)
     if f(M, N, K, sm_count, ctypes.byref(width), ctypes.byref(slices), ctypes.byref(cycles)) != 0:
@@ -331,7 +331,7 @@ def _act_plan(M: int, N: int, K: int, sm_count: int, float_out: bool = False):
     _, columns, cut = other[:3]
     blocks = -(-K // 64)
     chain = -(-blocks // cut)
-    if float_out and 64 * chain > 1536:
+    if float_out and 64 * chain > 768:
         return pairs
     others_us = 3 + 0.33 * chain * (1 if cut & (cut - 1) == 0 else 2) + 0.1 * -(-columns // cut)
     return pairs if cycles.value / 1520 + 2.2 < others_us else (False, columns, cut)

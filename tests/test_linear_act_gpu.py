@@ -2,7 +2,7 @@
 
 Tolerance. The product is off by at most 2e-6 of its conditioning c = |x| . |w| (as for the other products on the tensor cores; the 32-bit ones stay
 below that too), and so is the sum with the bias. An activation passes it on times its slope: at most 1.13 (gelu), for relu
-squared 2 |z|. Its own evaluation is off by less than 4 x 2^-24 of the result's size and, where it is z sigmoid(y), by 2^-23 |y| of it, with |y| at
+squared 2 |z|. Its own evaluation is off by less than 4 x 2^-24 of the result's size (gelu's own fit 24 x 2^-24) and, where it is z sigmoid(y), by 2^-23 |y| of it, with |y| at
 most 16 where the result is above 2^-23 of |z|: 2^-18 of |result| covers both. At the end one rounding: half a step.
 """
 import itertools

@@ -85,7 +85,7 @@ def test_plans_of_few_rows(M, N, K):
             assert width % 32 == 0 and 32 <= width <= 256 and slices in (1, 2, 4)
         else:
             assert width in (16, 32, 64, 128) and 1 <= slices <= 8
-            assert not float_out or -(-(-(-K // 64)) // slices) * 64 <= 1536, "a long chain of float sums"
+            assert not float_out or -(-(-(-K // 64)) // slices) * 64 <= 768, "a long chain of float sums"
 
 
 @pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 151936), (18, 151936), (19, 151936), (74, 151936), (75, 50257), (149, 151936), (5000, 300)])
