@@ -347,13 +347,12 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], a
     if x.dtype is torch.float32:
         if code != 0:
             return False
-        if _f32_act_on_tensor_cores(M, N, K):
-            cut = _f32_cut_plan(M, N, K, st.sm_count)
-            if cut is None:
-                _call(_act_fn("lin32_tc"), *same, st.sm_count, 1, act, st.status.data_ptr(), _stream())
-            else:
-                scratch = x.new_empty((cut[1],), dtype=torch.uint8)
-                _call(_act_fn("lin32_cut"), *same, act, cut[0], scratch.data_ptr(), st.sm_count, st.status.data_ptr(), _stream())
+        cut = _f32_cut_plan(M, N, K, st.sm_count)
+        if cut is not None:
+            scratch = x.new_empty((cut[1],), dtype=torch.uint8)
+            _call(_act_fn("lin32_cut"), *same, act, cut[0], scratch.data_ptr(), st.sm_count, st.status.data_ptr(), _stream())
+        elif _f32_act_on_tensor_cores(M, N, K):
+            _call(_act_fn("lin32_tc"), *same, st.sm_count, 1, act, st.status.data_ptr(), _stream())
         else:
             _call(_act_fn("lin32"), *same, 0, st.sm_count, 1, act, _stream())
         return True
@@ -394,11 +393,20 @@ def _f32_cut_plan(M: int, N: int, K: int, sm_count: int) -> Optional[tuple]:
     """(Tile width, bytes of scratch) where a product of floats on the tensor cores cuts its operands into bfloat16 numbers beforehand; None where it
     cuts them on its way, which takes less by the two kernels' estimates: measured (beforehand, on its way; us) 301 x 2301 x 1000 29 and 39,
     333 x 32003 x 1000 207 and 297, 2000 x 4000 x 2000 172 and 338, 512 x 1536 x 8960 144 and 172, 129 x 8960 x 1536 61 and 66; but 128 x 8960 x 1536
-    61 and 43, 129 x 1000 x 1000 25 and 18, 256 x 1536 x 8960 133 and 107."""
+    61 and 43, 129 x 1000 x 1000 25 and 18, 256 x 1536 x 8960 133 and 107. Below 128 columns or elements of K only multiply-adds are in its place:
+    (beforehand, multiply-adds) 1594 x 910 x 105 17 and 29, 2054 x 3014 x 65 38 and 66, 4000 x 100 x 2000 48 and 82, 367 x 64 x 995 23 and 31; but
+    2000 x 2000 x 16 25 and 25, 2703 x 265 x 80 17 and 13, 65 x 18000 x 100 36 and 23."""
+    if N < 128 or K < 128:
+        if M < 256 or M * N * K < (20_000_000 if K >= 256 else 100_000_000):
+            return None
+    elif not _f32_act_on_tensor_cores(M, N, K):
+        return None
     width, nbytes, ns = c_int(), c_int64(), c_int64()
     f = _fn("lin32_cut", "ib_linear_f32_cut_plan", [c_int64] * 3 + [c_int] + [c_void_p] * 3)
     if f(M, N, K, sm_count, ctypes.byref(width), ctypes.byref(nbytes), ctypes.byref(ns)) != 0 or nbytes.value > F32_CUT_SCRATCH:
         return None
+    if N < 128 or K < 128:
+        return width.value, nbytes.value
     other = _fn("lin32_tc", "ib_linear_f32_tc_ns", [c_int64] * 3 + [c_int], _ACT, c_int64)
     return (width.value, nbytes.value) if ns.value < other(M, N, K, sm_count) else None
 

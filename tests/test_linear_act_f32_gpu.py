@@ -100,7 +100,8 @@ def test_rows_and_results_that_start_anywhere():
 
 
 @pytest.mark.parametrize("M,N,K,cut", [(301, 2301, 1000, True), (1024, 1024, 1024, True), (500, 5003, 1000, True), (129, 1000, 1000, False), (257, 128, 16000, False),
-                                       (64, 3000, 1000, False), (300, 1000, 17000, False)])
+                                       (64, 3000, 1000, False), (300, 1000, 17000, False),
+                                       (2054, 3014, 65, True), (1000, 100, 500, True), (300, 300, 100, False), (65, 18000, 100, False)])
 def test_the_kernel_that_a_product_takes(M, N, K, cut):
     from infer_b200 import ops
     x, w, bias, res = _operands(M, N, K, torch.float32)
