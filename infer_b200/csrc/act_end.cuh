@@ -2,6 +2,7 @@
 // end of a tile: bias, activation, residual, one rounding, coalesced stores.
 #pragma once
 #include "common.cuh"
+#include "last_uses.h"
 #include "score.cuh"
 #include "tc_ops.cuh"
 
@@ -15,7 +16,8 @@ __device__ __forceinline__ void fence_barrier_init() { asm volatile("fence.mbarr
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// The same without handing memory over: nothing that a thread has written need be seen, so none waits for its stores (3,000 cycles behind a tile's).
+// The same without handing memory over: no thread waits for its stores (3,000 cycles behind a tile's). It orders no arrival on another CTA's barrier either:
+// before a CTA may end behind it, each barrier's last uses must have been waited for in the CTA that has it (last_uses).
 __device__ __forceinline__ void cluster_meet() {
     asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }

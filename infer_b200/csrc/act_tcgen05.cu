@@ -125,10 +125,12 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                     if (++s == STAGES) { s = 0; parity ^= 1u; }
                 }
             }
-            // No copy may land after the CTA is gone: the first CTA waits for every stage it was told of. (Without a failure
-            // the MMAs, which waited for them, have ended before the last barrier below.)
-            if (slots[1] && rank == 0)
-                for (int i = it > STAGES ? it - STAGES : 0; i < it; i++) mbar_wait(full_bar(i % STAGES), (i / STAGES) & 1);
+            // What another CTA sends here lands before this one ends: the commits that free the last stages, and where a wait ran out the copies
+            // of every stage that the first CTA was told of. (Without a failure the MMAs waited for those.)
+            if (!slots[1] && !ib::last_uses(it, STAGES, [&](int b, uint32_t phase) { return mbar_wait(empty_bar(b), phase); })) {
+                atomicExch(p.status, STATUS_TIMEOUT_PRODUCER); slots[1] = 1;
+            }
+            if (slots[1] && rank == 0) ib::last_uses(it, STAGES, [&](int b, uint32_t phase) { mbar_wait(full_bar(b), phase); return true; });
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -168,9 +170,13 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                     if (++s == STAGES) { s = 0; parity ^= 1u; }
                 }
             }
+            ib::pdl_launch_dependents();
+            // (the other CTA's warps have said of each accumulator that they have read it)
+            ok = ok && ib::last_uses(use, 2, [&](int b, uint32_t phase) { return mbar_wait_each(acc_empty_bar(b), phase); });
             if (!ok && lane == 0) { atomicExch(p.status, STATUS_TIMEOUT_MMA); slots[1] = 1; }
+        } else {
+            ib::pdl_launch_dependents();
         }
-        ib::pdl_launch_dependents();
         __syncwarp();
     } else {
         // ---------------------------------------------------------------- epilogue: a row of the CTA and half of the columns a thread
@@ -231,7 +237,7 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
         __syncwarp();
     }
     if constexpr (S > 1) {
-        cluster_meet();                                  // every MMA of the cluster is done: the rings are free
+        cluster_sync();                                  // every MMA of the cluster is done: the rings are free
         // [slice][group of four columns][row][4] of the columns that this CTA owns: width / S from width / S * slice on (32 bytes behind each
         // group: lanes that read two rows of four groups do not meet in a bank)
         const int own = p.width / S, quad = warp & 3, r = quad * 32 + lane, half = (warp - 2) >> 2, cols = p.width / 2;
@@ -299,7 +305,10 @@ act_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     }
     tc_fence_before();
     __syncthreads();
-    cluster_meet();                                      // no CTA's shared memory is needed by another any more
+    // No CTA's shared memory is needed by another any more: what was sent to this one's barriers has been waited for above, the slices' columns were at
+    // their barrier. Where a wait ran out that is not so, and what was sent before is ordered by the barrier itself.
+    if (slots[1]) cluster_sync();
+    else cluster_meet();
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(uint32_t(TMEM_COLS)) : "memory");

@@ -165,9 +165,12 @@ cut_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                     if (++s == STAGES) { s = 0; parity ^= 1u; }
                 }
             }
-            // No copy may land after the CTA is gone: the first CTA waits for every stage it was told of.
-            if (slots[1] && rank == 0)
-                for (int i = it > STAGES ? it - STAGES : 0; i < it; i++) mbar_wait(full_bar(i % STAGES), (i / STAGES) & 1);
+            // What another CTA sends here lands before this one ends: the commits that free the last stages, and where a wait ran out the copies
+            // of every stage that the first CTA was told of.
+            if (!slots[1] && !ib::last_uses(it, STAGES, [&](int b, uint32_t phase) { return mbar_wait(empty_bar(b), phase); })) {
+                atomicExch(p.status, STATUS_TIMEOUT_PRODUCER); slots[1] = 1;
+            }
+            if (slots[1] && rank == 0) ib::last_uses(it, STAGES, [&](int b, uint32_t phase) { mbar_wait(full_bar(b), phase); return true; });
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -227,9 +230,16 @@ cut_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                     if (++s == STAGES) { s = 0; parity ^= 1u; }
                 }
             }
+            ib::pdl_launch_dependents();
+            // (the other CTA's warps have said of each accumulator that they have read it)
+            ok = ok && ib::last_uses(use, 2, [&](int b, uint32_t phase) { return mbar_wait_each(main_empty(b), phase); });
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                if (ok && (used >> i & 1)) ok = mbar_wait_each(small_empty(i), (turn >> i & 1) ^ 1);
             if (!ok && lane == 0) { atomicExch(p.status, STATUS_TIMEOUT_MMA); slots[1] = 1; }
+        } else {
+            ib::pdl_launch_dependents();
         }
-        ib::pdl_launch_dependents();
         __syncwarp();
     } else {
         // ---------------------------------------------------------------- epilogue: a row and the tile's columns a thread
@@ -317,7 +327,10 @@ cut_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     }
     tc_fence_before();
     __syncthreads();
-    cluster_meet();                                      // neither CTA's shared memory is needed by the other any more
+    // Neither CTA's shared memory is needed by the other any more: what was sent to this one's barriers has been waited for above. Where a wait ran out
+    // that is not so, and what was sent before is ordered by the barrier itself.
+    if (slots[1]) cluster_sync();
+    else cluster_meet();
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(uint32_t(TMEM_COLS)) : "memory");
