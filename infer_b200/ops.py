@@ -304,6 +304,9 @@ def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, seed: torch
 
 # ----------------------------------------------------------------------------- log probabilities
 
+MAX_ALTERNATIVES = 20        # that can be asked for at a place
+
+
 class TokenLogprobs(NamedTuple):
     """What ``token_logprobs`` and ``head_logprobs`` return, one row a place: float32 [T], float32 [T], int32 [T, top], float32 [T, top]."""
     logprob: torch.Tensor

@@ -1,0 +1,13 @@
+"""Scores: what is refused, and that it is refused before anything has run (no GPU is needed)."""
+from types import SimpleNamespace
+
+import pytest
+
+
+@pytest.mark.parametrize("top", [21, -1, 1000])
+def test_step_logprobs_refuses_alternatives_before_it_looks_at_the_step(top):
+    from infer_b200.engine import Engine
+    eng = object.__new__(Engine)                     # no cache, no model: whatever the call did with them would be another error
+    eng.spec = SimpleNamespace(vocab_size=50)
+    with pytest.raises(ValueError, match="alternatives"):
+        eng.step_logprobs([("r", [1, 2], [0, 1])], [1, 2], top)

@@ -1,0 +1,40 @@
+"""Scores of designs that keep a state per request: a refused call leaves pages, lengths and states as they were."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _llm(preset, **kw):
+    from infer_b200.config import parse_config
+    from infer_b200.engine.generation import LLM
+    from infer_b200.models import load_preset
+    from infer_b200.weights import random_weights
+    arch, typed = parse_config(load_preset(preset))
+    spec = arch.to_spec(typed)
+    return LLM(None, dtype="bfloat16", spec=spec, weights=random_weights(spec, 3, torch.bfloat16), slots=2, max_seq=128, **kw)
+
+
+@pytest.mark.parametrize("preset", ["tiny-fozerax", "tiny-ruvenex", "tiny-b"])
+def test_a_refused_step_changes_nothing(preset):
+    eng = _llm(preset).engine
+    ids = np.random.default_rng(1).integers(0, eng.spec.vocab_size, 40).tolist()
+
+    def portions(rid, refused):
+        got = []
+        eng.add_request(rid)
+        for lo, hi in ((0, 20), (20, 39)):
+            entry = [(rid, ids[lo:hi], list(range(hi - lo)))]
+            if refused:
+                free, length = eng.cache.pages_free(), eng.cache.length(rid)
+                for asked, top in ((ids[lo + 1:hi + 1], 21), (ids[lo + 1:hi + 1], -1), (ids[lo + 1:hi], 3), ([eng.spec.vocab_size] * (hi - lo), 3)):
+                    with pytest.raises(ValueError):
+                        eng.step_logprobs(entry, asked, top)
+                    assert eng.cache.pages_free() == free and eng.cache.length(rid) == length and eng.cache.requests[rid].reserved == length
+            got.append(eng.step_logprobs(entry, ids[lo + 1:hi + 1], 3))
+        eng.end_request(rid)
+        return [torch.cat(t) for t in zip(*got)]
+    plain, after = portions("a", False), portions("b", True)
+    assert all(torch.equal(x, y) for x, y in zip(plain, after))
+    eng.check_status()
