@@ -327,10 +327,15 @@ def _plain_tokens(tokens: torch.Tensor, rows: int, device) -> bool:
     return tokens.dtype is torch.int32 and tokens.device == device and tokens.shape == (rows,) and tokens.is_contiguous()
 
 
+def distribution_in_range(scale: float, softcap: float) -> bool:
+    """Whether ``token_logprobs`` and ``head_logprobs`` take this scale and cap."""
+    return 1e-18 <= scale <= 1e18 and (softcap == 0 or 1e-18 <= softcap <= 1e18)
+
+
 def _refuse_distribution(top: int, scale: float, softcap: float) -> None:
     """(The bounds keep scale / softcap, which the kernels multiply by, a float32 number.)"""
-    if not 0 <= top <= 20:
-        raise KernelError(f"0 to 20 alternatives can be asked for, not {top}")
+    if not 0 <= top <= MAX_ALTERNATIVES:
+        raise KernelError(f"0 to {MAX_ALTERNATIVES} alternatives can be asked for, not {top}")
     if not 1e-18 <= scale <= 1e18:
         raise KernelError(f"the logits' scale must lie between 1e-18 and 1e18, not be {scale}")
     raise KernelError(f"the logits' cap must lie between 1e-18 and 1e18, or be 0 for none, not {softcap}")
@@ -365,7 +370,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     tensors of the result's shapes to write into.
     Each call may run on any stream; a captured one reads its inputs anew at each replay. The same call gives the same bits; a row's last bits
     may differ where it lies otherwise to 16 bytes or among another number of rows."""
-    if not (0 <= top <= 20 and 1e-18 <= scale <= 1e18 and (softcap == 0 or 1e-18 <= softcap <= 1e18)):
+    if not (0 <= top <= MAX_ALTERNATIVES and distribution_in_range(scale, softcap)):
         _refuse_distribution(top, scale, softcap)
     if not logits.is_cuda or logits.dtype is not torch.float32 or not logits.is_contiguous():
         _check(logits, "logits", torch.float32)
@@ -408,7 +413,7 @@ def head_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[torch.Tenso
     not kept: bfloat16 rows go through a kernel that holds them in tensor memory only; up to 8 rows, rows that do not keep to 16 bytes and
     float32 go through logits of a few rows at a time. ``w`` is a loaded weight (as for ``linear``). A kernel whose bounded wait runs out
     says so in the device's status word."""
-    if not (0 <= top <= 20 and 1e-18 <= scale <= 1e18 and (softcap == 0 or 1e-18 <= softcap <= 1e18)):
+    if not (0 <= top <= MAX_ALTERNATIVES and distribution_in_range(scale, softcap)):
         _refuse_distribution(top, scale, softcap)
     _check_product("head_logprobs", x, w)
     (T, K), V, device = x.shape, w.shape[0], x.device

@@ -108,9 +108,9 @@ class LinearHead(Head):
         self.linear = Linear.share(self.rt, table)
 
     def logprobs(self, x, tokens, top, status=None):
-        # (a subclass or an instance with logits of its own goes by those)
+        # (a subclass or an instance with logits of its own goes by those, and so does a scale or cap that the operator does not take)
         if type(self).forward is not LinearHead.forward or "forward" in vars(self) or type(self.linear) is not Linear or self.linear.bias is not None \
-                or not self.rt.fast("linear"):
+                or not ops.distribution_in_range(self.logit_scale, self.softcap) or not self.rt.fast("linear"):
             return super().logprobs(x, tokens, top, status)
         return ops.head_logprobs(x, self.linear.weight, tokens, top, self.logit_scale, self.softcap, status)
 

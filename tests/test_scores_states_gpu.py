@@ -38,3 +38,21 @@ def test_a_refused_step_changes_nothing(preset):
     plain, after = portions("a", False), portions("b", True)
     assert all(torch.equal(x, y) for x, y in zip(plain, after))
     eng.check_status()
+
+
+@pytest.mark.parametrize("scale,cap", [(-0.5, 0.0), (1e-20, 0.0), (-1.0, 20.0), (2.0, 1e20)])
+def test_a_head_whose_scale_the_operator_does_not_take_is_scored_by_its_logits(scale, cap):
+    """Against the engine's own logits: the same kernel on the same logits, so the same bits."""
+    from infer_b200 import ops
+    eng = _llm("tiny-b").engine
+    head = eng.model.head
+    head.logit_scale, head.softcap = scale, cap
+    ids = np.random.default_rng(2).integers(0, eng.spec.vocab_size, 30).tolist()
+    eng.add_request("r")
+    got = eng.step_logprobs([("r", ids[:-1], list(range(29)))], ids[1:], 4)
+    eng.end_request("r")
+    eng.add_request("s")
+    logits = eng.step([("s", ids[:-1], list(range(29)))])
+    eng.end_request("s")
+    want = ops.token_logprobs(logits, torch.tensor(ids[1:], dtype=torch.int32, device=logits.device), 4)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and got.logprob.isfinite().all()
