@@ -38,7 +38,7 @@ class PendingTokens:
             return {}
         self._event.synchronize()
         logprob, entropy, ids, best = (t.tolist() for t in self._scores)
-        return {rid: TokenScore(logprob[i], entropy[i], [(t, p) for t, p in zip(ids[i][:n], best[i][:n]) if t >= 0])
+        return {rid: TokenScore(logprob[i], entropy[i], [(t, p) for t, p in zip(ids[i][:int(n)], best[i][:int(n)]) if t >= 0])
                 for i, (rid, n) in enumerate(zip(self.rids, self._asked)) if n is not None}
 
 
@@ -113,7 +113,7 @@ class GenerationEngine(BatchEngine):
         logits = self.engine.step(entries)
         with torch.cuda.device(self.engine.rt.device):
             ids = self.sampler.sample(logits, [b.sample for b in rows], [b.position for b in rows], self.engine.next_tokens, slots)
-            scores = ops.token_logprobs(logits, ids, max(n for n in asked if n is not None))
+            scores = ops.token_logprobs(logits, ids, max(int(n) for n in asked if n is not None))
             copies = []
             for t in (ids, *scores):
                 host = torch.empty(t.shape, dtype=t.dtype, pin_memory=True)

@@ -232,7 +232,7 @@ class Scheduler:
     def submit(self, r: Request) -> None:
         if not r.prompt:
             raise ValueError(f"request {r.id!r}: empty prompt")
-        if r.sample.logprobs is not None and not 0 <= r.sample.logprobs <= 20:
+        if r.sample.logprobs is not None and r.sample.logprobs not in range(21):         # (no fraction)
             raise ValueError(f"request {r.id!r}: 0 to 20 alternatives can be asked for, not {r.sample.logprobs}")
         total = len(r.prompt) + r.max_new
         limit = min(self.eng.max_seq_len, self.eng.capacity_tokens())
