@@ -14,12 +14,6 @@ __device__ __forceinline__ float exp2_fast(float x) {        // 2^-inf = 0, abou
     return y;
 }
 
-// What a product's sum z is as a logit. A masked one, -inf (also what stands for places outside the vocabulary), stays masked under a cap.
-__device__ __forceinline__ float logit(float z, float scale, float cap) {
-    const float l = z * scale;
-    return cap > 0.0f && l != -INFINITY ? cap * tanhf(l / cap) : l;
-}
-
 template <int N> __device__ __forceinline__ float largest_of(const float (&z)[N]) {
     float top = z[0];
 #pragma unroll
@@ -27,31 +21,47 @@ template <int N> __device__ __forceinline__ float largest_of(const float (&z)[N]
     return top;
 }
 
-// The logits of N sums under a cap, without tanhf's branches: for |u| <= 0.6 an odd polynomial (a minimax fit of tanh(u) / u in u^2, off by
-// 2.5e-9 before its roundings: 2 x 2^-24 of the result with them), else 1 - 2 / (1 + e^2|u|) (5 x 2^-24). A thread goes by the largest of its own, one whose
-// results are not needed (`counts`) by the polynomial.
+// The logit of a product's sum z under a cap, cap tanh(u) with u = z scale / cap: a value of z is the same logit wherever it is evaluated, in the sums, as the asked
+// token or as an alternative, so that a token with nearly all the probability keeps its digits and is never likelier than 1. (No product here may be
+// contracted into a sum that follows: __fmul_rn.)
+// From |u| = 0.6 on tanh u = 1 - 2 / (1 + e^2u): beyond atanh(1/2) = 0.55 what is subtracted is below 1/2, so no digits cancel (5 x 2^-24 of the result).
+// Below, an odd polynomial, a minimax fit of tanh(u) / u in u^2 made for this place, of the degree at which its error over [0, 0.6], 4.9e-9 with the
+// constants as they are stored, is below its roundings (2 x 2^-24 with them).
+constexpr float TANH_SPLIT = 0.6f;
+__device__ __forceinline__ float tanh_below(float u) {
+    const float q = u * u;
+    float t = fmaf(q, -0.005852164700627327f, 0.02075362578034401f);
+    t = fmaf(q, t, -0.05376870185136795f);
+    t = fmaf(q, t, 0.13331688940525055f);
+    t = fmaf(q, t, -0.3333328366279602f);
+    t = fmaf(q, t, 1.0f);
+    return __fmul_rn(u, t);
+}
+__device__ __forceinline__ float tanh_above(float u) {
+    return copysignf(1.0f - __fdividef(2.0f, 1.0f + exp2_fast(__fmul_rn(fabsf(u), 2.0f * LOG2E))), u);
+}
+// (Both forms, then a choice: as two sides of a condition they became a branch for each element, 647 us at 512 rows x 1536 against 152,064 under a cap of 10; so 359.)
+__device__ __forceinline__ float cap_tanh(float u, float cap) {
+    const float below = tanh_below(u), above = tanh_above(u);
+    return __fmul_rn(cap, fabsf(u) <= TANH_SPLIT ? below : above);
+}
+// A masked sum, -inf (also what stands for places outside the vocabulary), stays masked.
+__device__ __forceinline__ float cap_logit(float z, float scale, float cap) {
+    const float u = __fmul_rn(z, scale / cap), l = cap_tanh(u, cap);
+    return u == -INFINITY ? u : l;
+}
+// N of them (`counts`: whether the thread's results are needed). Where a thread's are all below the split, as a model's are, the second form is left out.
 template <int N> __device__ __forceinline__ void cap_logits(float (&l)[N], const float (&z)[N], float scale, float cap, bool counts = true) {
     const float to_u = scale / cap;
     float most = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; i++) { l[i] = z[i] * to_u; most = fmaxf(most, l[i] == -INFINITY ? 0.0f : fabsf(l[i])); }
-    if (most <= 0.6f || !counts) {
+    for (int i = 0; i < N; i++) { l[i] = __fmul_rn(z[i], to_u); most = fmaxf(most, l[i] == -INFINITY ? 0.0f : fabsf(l[i])); }
+    if (most <= TANH_SPLIT || !counts) {
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const float u = l[i], q = u * u;
-            float t = fmaf(q, -0.005852164700627327f, 0.02075362578034401f);
-            t = fmaf(q, t, -0.05376870185136795f);
-            t = fmaf(q, t, 0.13331688940525055f);
-            t = fmaf(q, t, -0.3333328366279602f);
-            t = fmaf(q, t, 1.0f);
-            l[i] = u == -INFINITY ? u : cap * (u * t);
-        }
+        for (int i = 0; i < N; i++) { const float t = __fmul_rn(cap, tanh_below(l[i])); l[i] = l[i] == -INFINITY ? l[i] : t; }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const float u = l[i], t = 1.0f - __fdividef(2.0f, 1.0f + exp2_fast(fabsf(u) * (2.0f * LOG2E)));
-            l[i] = u == -INFINITY ? u : cap * copysignf(t, u);
-        }
+        for (int i = 0; i < N; i++) { const float t = cap_tanh(l[i], cap); l[i] = l[i] == -INFINITY ? l[i] : t; }
     }
 }
 
@@ -98,7 +108,7 @@ __device__ __forceinline__ Stats warp_join(Stats v) {
 
 // (at: the token's sum z)
 __device__ __forceinline__ float logprob_of(const Stats& st, float z, float scale, float cap) {
-    return cap > 0.0f ? st.logprob(logit(z, scale, cap)) : st.logprob(z, scale);
+    return cap > 0.0f ? st.logprob(cap_logit(z, scale, cap)) : st.logprob(z, scale);
 }
 __device__ __forceinline__ void finish(const Stats& st, int token, float at, float scale, float cap, int64_t vocab, float* logprob, float* entropy, int* status) {
     if (entropy) *entropy = st.entropy();
