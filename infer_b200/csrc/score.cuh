@@ -45,23 +45,23 @@ __device__ __forceinline__ float cap_tanh(float u, float cap) {
     const float below = tanh_below(u), above = tanh_above(u);
     return __fmul_rn(cap, fabsf(u) <= TANH_SPLIT ? below : above);
 }
-// A masked sum, -inf (also what stands for places outside the vocabulary), stays masked.
+// A masked sum, -inf (also what stands for places outside the vocabulary), stays masked; a finite one never is, whatever its product with scale / cap. +inf: the cap.
 __device__ __forceinline__ float cap_logit(float z, float scale, float cap) {
-    const float u = __fmul_rn(z, scale / cap), l = cap_tanh(u, cap);
-    return u == -INFINITY ? u : l;
+    const float l = cap_tanh(__fmul_rn(z, scale / cap), cap);
+    return z == -INFINITY ? z : l;
 }
 // N of them (`counts`: whether the thread's results are needed). Where a thread's are all below the split, as a model's are, the second form is left out.
 template <int N> __device__ __forceinline__ void cap_logits(float (&l)[N], const float (&z)[N], float scale, float cap, bool counts = true) {
     const float to_u = scale / cap;
     float most = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; i++) { l[i] = __fmul_rn(z[i], to_u); most = fmaxf(most, l[i] == -INFINITY ? 0.0f : fabsf(l[i])); }
+    for (int i = 0; i < N; i++) { l[i] = __fmul_rn(z[i], to_u); most = fmaxf(most, z[i] == -INFINITY ? 0.0f : fabsf(l[i])); }
     if (most <= TANH_SPLIT || !counts) {
 #pragma unroll
-        for (int i = 0; i < N; i++) { const float t = __fmul_rn(cap, tanh_below(l[i])); l[i] = l[i] == -INFINITY ? l[i] : t; }
+        for (int i = 0; i < N; i++) { const float t = __fmul_rn(cap, tanh_below(l[i])); l[i] = z[i] == -INFINITY ? z[i] : t; }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; i++) { const float t = cap_tanh(l[i], cap); l[i] = l[i] == -INFINITY ? l[i] : t; }
+        for (int i = 0; i < N; i++) { const float t = cap_tanh(l[i], cap); l[i] = z[i] == -INFINITY ? z[i] : t; }
     }
 }
 

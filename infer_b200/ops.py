@@ -364,7 +364,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     (int32 [T]; -1 or no ``tokens`` at all: none is asked for, the result is 0), the entropy of the row's distribution, and the ``top``
     likeliest tokens (0 to 20) with their log probabilities, by falling logit, among equal logits the lowest id first. A logit of -inf has no
     probability and is no alternative; places without an alternative hold id -1 and -inf. A row of -inf only: log probability -inf,
-    entropy 0. A NaN or +inf in a row makes its floats NaN (the ids follow the logits that are no NaN). Any other token outside
+    entropy 0. A NaN in a row, or without a cap a +inf, makes its floats NaN (the ids follow the logits that are no NaN); under a cap +inf is the cap. Any other token outside
     [0, V): NaN, and the status word (if given) is set to 1. ``scale`` / ``softcap``: the distribution is that of
     softcap * tanh(logits * scale / softcap) (-inf stays -inf), or logits * scale without a cap; alternatives go by ``logits``. ``out``: contiguous
     tensors of the result's shapes to write into.

@@ -1,4 +1,5 @@
-"""Log probabilities under a cap: a value is the same logit wherever the kernels evaluate it, so that a token that is all but certain keeps its digits.
+"""Log probabilities under a cap: a value is the same logit wherever the kernels evaluate it, so that a token that is all but certain keeps its digits; and values
+whose product with scale / cap is no float32 number.
 
 Tolerances. A logit cap tanh(u): u = z (scale / cap) carries two roundings, 2 x 2^-24 |u|, of which tanh keeps at most |u| / cosh^2 u < 0.45 of its size; tanh itself
 5 x 2^-24, the product with the cap one more: off by less than 7 x 2^-24 cap. Where a token's probability is p, the others' share S - 1 of the sum S is at
@@ -7,10 +8,12 @@ most (1 - p) / p, and an error of 7 x 2^-24 cap in each difference l - m moves i
 most 10 within the token's group of 16 and 2 groups behind it, 10 in the block and 5 among a row's CTAs from logits, 18 within the token's group of 32 columns, 16 groups
 behind it, 19 chunks a lane and 5 lanes from a head's rows: below 60 x 2^-24. The logarithm of a number next to 1 rounds once more.
 """
+import math
+
 import pytest
 import torch
 
-from test_logprobs_gpu import DEV, STEP
+from test_logprobs_gpu import DEV, STEP, check
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +54,22 @@ def test_a_sure_token_keeps_its_digits(cap, scale):
         for top in (0, 4):
             r = ops.head_logprobs(x, w, th, top, scale=scale, softcap=cap)
             _sure(r, cap * torch.tanh(zh * scale / cap), th, cap)
+
+
+@pytest.mark.parametrize("V", [40, 8200, 50257])
+@pytest.mark.parametrize("scale,cap", [(2.0, 0.5), (1.0, 30.0), (4.0, 30.0), (1e18, 1e-18), (1.0, 0.25)])
+def test_values_whose_product_is_no_float(V, scale, cap):
+    """Masks of the type's lowest value are finite logits: -cap under a cap; +inf is the cap; -inf stays masked, a NaN is one."""
+    from infer_b200 import ops
+    inf, low = math.inf, torch.finfo(torch.float32).min
+    g = torch.Generator(device=DEV).manual_seed(V)
+    n = lambda: torch.randn(V, device=DEV, generator=g)
+    every = torch.arange(V, device=DEV)
+    rows = [torch.full((V,), low, device=DEV), n().masked_fill(every % 3 == 1, low), n().masked_fill(every % 3 == 1, low).masked_fill(every % 3 == 2, -inf),
+            n().masked_fill(every % 5 == 1, -low).masked_fill(every % 5 == 2, inf), torch.full((V,), -inf, device=DEV),
+            n().masked_fill(every == V // 2, math.nan), torch.full((V,), -inf, device=DEV).masked_fill(every == 3, low), torch.full((V,), inf, device=DEV)]
+    z = torch.stack(rows)
+    l = cap * torch.tanh(z.double() * scale / cap).masked_fill(z == -inf, -inf)
+    t = torch.arange(len(rows), device=DEV, dtype=torch.int32) % V
+    for top in (0, 7):
+        check(ops.token_logprobs(z, t, top, scale=scale, softcap=cap), l, z, t, top, 7 * STEP * cap)
