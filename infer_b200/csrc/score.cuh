@@ -90,9 +90,11 @@ struct Stats {
         s += s0 + s1;
         d += d0 + d1;
     }
-    // of the logit z scale: its distance from m is formed as add() formed the others'
+    // of the logit z scale: its distance from m is formed as add() formed the others'. (A scale leaves it half a step above the largest one's, that of the rounded
+    // m: no token is likelier than 1.)
     __device__ __forceinline__ float logprob(float z, float scale = 1.0f) const {
-        return m == -INFINITY && s == 0.0f ? -INFINITY : fmaf(z, scale, -m) - logf(s);
+        const float l = fmaf(z, scale, -m) - logf(s);
+        return m == -INFINITY && s == 0.0f ? -INFINITY : l > 0.0f ? 0.0f : l;
     }
     __device__ __forceinline__ float entropy() const { return m == -INFINITY && s == 0.0f ? 0.0f : logf(s) - d / s; }
 };

@@ -56,6 +56,17 @@ def test_a_sure_token_keeps_its_digits(cap, scale):
             _sure(r, cap * torch.tanh(zh * scale / cap), th, cap)
 
 
+def test_no_token_is_likelier_than_one_without_a_cap():
+    from infer_b200 import ops
+    g = torch.Generator(device=DEV).manual_seed(9)
+    z = torch.randn(2000, 500, device=DEV, generator=g) - 60
+    t = torch.randint(0, 500, (2000,), device=DEV, generator=g, dtype=torch.int32)
+    z[torch.arange(2000, device=DEV), t.long()] = 40 + 20 * torch.rand(2000, device=DEV, generator=g)
+    for scale in (1.0, 0.7, 1.3):
+        r = ops.token_logprobs(z, t, 1, scale=scale)
+        assert (r.logprob <= 0).all() and (r.logprob >= -4 * STEP).all() and torch.equal(r.logprob, r.top_logprobs[:, 0])
+
+
 @pytest.mark.parametrize("V", [40, 8200, 50257])
 @pytest.mark.parametrize("scale,cap", [(2.0, 0.5), (1.0, 30.0), (4.0, 30.0), (1e18, 1e-18), (1.0, 0.25)])
 def test_values_whose_product_is_no_float(V, scale, cap):
