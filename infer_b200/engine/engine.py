@@ -487,8 +487,8 @@ class Engine:
     def step_logprobs(self, entries: Sequence[StepEntry], tokens: Sequence[int], top: int = 0) -> "ops.TokenLogprobs":
         """As ``step``, but in place of logits it returns how likely ``tokens`` (one id per wanted place, in the order of the entries and of
         their ``want`` lists; -1: none) are there, the entropy at each place and the ``top`` likeliest tokens, on the device
-        (``ops.token_logprobs`` says exactly what). The logits are not stored, so that every place of a long portion may be wanted. Arguments that
-        cannot be served are refused before anything is reserved or run."""
+        (``ops.token_logprobs`` says exactly what). Of a bfloat16 head the logits are not stored, of others 1 GB at a time, so that every place of a long
+        portion may be wanted. Arguments that cannot be served are refused before anything is reserved or run."""
         if not 0 <= int(top) <= ops.MAX_ALTERNATIVES:
             raise ValueError(f"0 to {ops.MAX_ALTERNATIVES} alternatives can be asked for, not {top}")
         tokens, top = [int(t) for t in tokens], int(top)

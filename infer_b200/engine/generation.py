@@ -208,7 +208,7 @@ class LLM:
 
     def score(self, prompts: Sequence[Sequence[int]], top: int = 0) -> List["PromptScore"]:
         """How likely the model finds given token ids: for each prompt of n ids a ``PromptScore`` of n - 1 places. Prompts run in portions under the
-        token budget, several in a step; the logits are not stored."""
+        token budget, several in a step; the logits are not stored (of a 32-bit model a portion's are for the moment)."""
         prompts = [[int(t) for t in p] for p in prompts]
         V = self.engine.spec.vocab_size
         for i, p in enumerate(prompts):

@@ -79,6 +79,10 @@ class TokenTable(Embedding):
         return rows
 
 
+# Logits that ``LinearHead.logprobs`` has in memory at a time where it needs them (float32 heads, plain products, a subclass's own): 1 GB.
+LOGPROB_LOGITS = 1 << 28
+
+
 @register_head("linear_head")
 class LinearHead(Head):
     def __init__(self, spec: PartSpec, runtime):
@@ -111,7 +115,11 @@ class LinearHead(Head):
         # (a subclass or an instance with logits of its own goes by those, and so does a scale or cap that the operator does not take)
         if type(self).forward is not LinearHead.forward or "forward" in vars(self) or type(self.linear) is not Linear or self.linear.bias is not None \
                 or not ops.distribution_in_range(self.logit_scale, self.softcap) or not self.rt.fast("linear"):
-            return super().logprobs(x, tokens, top, status)
+            rows = max(1, LOGPROB_LOGITS // self.vocab)
+            if len(x) <= rows:
+                return super().logprobs(x, tokens, top, status)
+            parts = [super(LinearHead, self).logprobs(x[lo:lo + rows], None if tokens is None else tokens[lo:lo + rows], top, status) for lo in range(0, len(x), rows)]
+            return ops.TokenLogprobs(*(torch.cat(part) for part in zip(*parts)))
         return ops.head_logprobs(x, self.linear.weight, tokens, top, self.logit_scale, self.softcap, status)
 
     def forward(self, x):

@@ -6,14 +6,14 @@ import torch
 pytestmark = pytest.mark.gpu
 
 
-def _llm(preset, **kw):
+def _llm(preset, dtype="bfloat16", **kw):
     from infer_b200.config import parse_config
     from infer_b200.engine.generation import LLM
     from infer_b200.models import load_preset
     from infer_b200.weights import random_weights
     arch, typed = parse_config(load_preset(preset))
     spec = arch.to_spec(typed)
-    return LLM(None, dtype="bfloat16", spec=spec, weights=random_weights(spec, 3, torch.bfloat16), slots=2, max_seq=128, **kw)
+    return LLM(None, dtype=dtype, spec=spec, weights=random_weights(spec, 3, torch.bfloat16), slots=2, max_seq=128, **kw)
 
 
 @pytest.mark.parametrize("preset", ["tiny-fozerax", "tiny-ruvenex", "tiny-b"])
@@ -56,3 +56,27 @@ def test_a_head_whose_scale_the_operator_does_not_take_is_scored_by_its_logits(s
     eng.end_request("s")
     want = ops.token_logprobs(logits, torch.tensor(ids[1:], dtype=torch.int32, device=logits.device), 4)
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and got.logprob.isfinite().all()
+
+
+@pytest.mark.parametrize("preset", ["tiny-a", "tiny-b", "tiny-pefazen"])
+@pytest.mark.parametrize("rows", [1, 7, 39])
+def test_a_32_bit_heads_logits_are_stored_for_some_rows_at_a_time(preset, rows, monkeypatch):
+    """The 32-bit products sum a row in the same order whatever the number of rows: the same bits."""
+    from infer_b200.parts import vocab
+    llm = _llm(preset, "float32")
+    V = llm.engine.spec.vocab_size
+    ids = np.random.default_rng(5).integers(0, V, 41).tolist()
+    want = llm.score([ids], top=3)[0]
+    monkeypatch.setattr(vocab, "LOGPROB_LOGITS", rows * V + V // 2)
+    head, seen = llm.engine.model.head, []
+    plain = type(head).forward
+
+    class Counted(type(head)):
+        def forward(self, x):
+            seen.append(len(x))
+            return plain(self, x)
+    head.__class__ = Counted
+    got = llm.score([ids], top=3)[0]
+    assert seen == [rows] * (40 // rows) + ([40 % rows] if 40 % rows else [])
+    for a, b in zip((want.logprobs, want.entropies, want.top_ids, want.top_logprobs), (got.logprobs, got.entropies, got.top_ids, got.top_logprobs)):
+        assert np.array_equal(a, b)
