@@ -459,12 +459,14 @@ ACTIVATIONS = {"none": 0, "relu": 1, "relu_squared": 2, "gelu_tanh": 3, "gelu": 
 
 
 def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: str = "none",
-               residual: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+               residual: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None,
+               plain: bool = False) -> torch.Tensor:
     """out = residual + act(x @ w.T + bias), rounded once. x [M, K], w [N, K], both bfloat16 or both float32; bias float32 [N]; residual float32
     [M, N] (may be ``out``); ``activation``: "none", "relu", "relu_squared" (max(z, 0)^2), "gelu_tanh"
     (0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3)))), "gelu" (0.5 z (1 + erf(z / sqrt 2))), "silu" (z / (1 + e^-z)). The result is
     float32 or bfloat16 (default: as x; with a residual float32). ``w`` is a loaded weight (as for ``linear``). A kernel whose bounded wait
-    runs out says so in the device's status word."""
+    runs out says so in the device's status word. Which kernel it is, and so the order of a row's sums, may depend on the number of rows; with ``plain`` it is
+    ``linear_plain``'s product, whose order does not, with the activation in a kernel behind it."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise KernelError(f"activation {activation!r} is not among {sorted(ACTIVATIONS)}")
@@ -481,13 +483,13 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
         _check_beside("out", out, out_dtype, (M, N), device)
     if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
-            return linear_act(x, w, bias, activation, residual, out_dtype, out)
+            return linear_act(x, w, bias, activation, residual, out_dtype, out, plain)
     if out is None:
         out = x.new_empty((M, N), dtype=out_dtype)
     if M == 0:
         return out
     from . import fast_ops
-    if fast_ops.linear_act(x, w, bias, act, residual, out, code):
+    if not plain and fast_ops.linear_act(x, w, bias, act, residual, out, code):
         return out
     # rows that do not keep to 16 bytes, float32 rows into a bfloat16 result: the float sums first, then what is left to do
     z = linear_plain(x, w, bias, None, torch.float32, w_ready=True)

@@ -57,7 +57,7 @@ class Linear(Watched):
         """x [rows, in] in the compute dtype (or a DeferredNorm of float32 rows). With ``residual`` (float32 [rows, out]) the result is
         float32 and is written over ``residual``. Otherwise the result has ``out_dtype`` (default:
         the compute dtype), and is written into ``out`` (contiguous [rows, out] of that dtype) if given. ``activation``: of the product and its
-        bias, before the residual, without a rounding between (``ops.linear_act`` names them)."""
+        bias, before the residual, without a rounding between (``ops.linear_act`` names them). In 32 bits a row's result does not depend on the other rows."""
         from .base import DeferredNorm
         if residual is not None:
             out, out_dtype = residual, torch.float32
@@ -65,7 +65,7 @@ class Linear(Watched):
             out_dtype = out.dtype
         if activation is not None:
             x = x.materialize() if isinstance(x, DeferredNorm) else x
-            return ops.linear_act(x, self.weight, self.bias, activation, residual, out_dtype or self.rt.dtype, out)
+            return ops.linear_act(x, self.weight, self.bias, activation, residual, out_dtype or self.rt.dtype, out, not self.rt.fast("linear"))
         if self.rt.fast("linear"):
             from .. import fast_ops
             y = fast_ops.linear(x, self.weight, self.bias, residual, out_dtype or self.rt.dtype, out)
