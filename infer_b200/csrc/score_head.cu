@@ -449,11 +449,16 @@ join_chunks_kernel(const JoinParams p) {
     }
     __syncthreads();
     const unsigned long long least = bound;
-    // (at most `top` lists: where there are more, as many as have a first key that reaches the top-th of them)
-    for (int c = threadIdx.x; c < p.chunks; c += JOIN_THREADS)
-        if (heads[c] >= least) chosen[atomicAdd(&n_chosen, 1)] = c;
+    // (at most `top` lists: where there are more, as many as have a first key that reaches the top-th of them. Where a wait of the kernel before ran out lists
+    // hold anything, the same key many times too: no more than `top` are taken.)
+    for (int c = threadIdx.x; c < p.chunks; c += JOIN_THREADS) {
+        if (heads[c] >= least) {
+            const int at = atomicAdd(&n_chosen, 1);
+            if (at < p.top) chosen[at] = c;
+        }
+    }
     __syncthreads();
-    const int n_keys = n_chosen * p.top;
+    const int n_keys = min(n_chosen, p.top) * p.top;
     constexpr int EACH = (MAX_TOP * MAX_TOP + JOIN_THREADS - 1) / JOIN_THREADS;
     unsigned long long key[EACH];                                       // (requested together, looked at afterwards)
 #pragma unroll
