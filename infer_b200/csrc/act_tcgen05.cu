@@ -383,11 +383,12 @@ IB_EXPORT int ib_linear_act_plan(int64_t M, int64_t N, int64_t K, int sms, int* 
             if (least < 0 || cost < least) { least = cost; *width = w; *slices = s; }
         }
     }
+    if (least < 0) return ib::fail(IB_ERR_ARG, "linear_act: too many tiles, or fewer than two SMs");
     // (as many tiles, but no wider than they need to be)
     const int64_t tn = (N + *width - 1) / *width;
     if (cycles) *cycles = least;
-    if (least >= 0) *width = int(((N + tn - 1) / tn + 31) / 32 * 32);
-    return least < 0 ? ib::fail(IB_ERR_ARG, "linear_act: too many tiles") : IB_OK;
+    *width = int(((N + tn - 1) / tn + 31) / 32 * 32);
+    return IB_OK;
 }
 
 // x [M, K], w [N, K] bfloat16 with 16-byte aligned bases, K a multiple of 8; bias float [N] or null; residual float [M, N] or null (may be out); act: an

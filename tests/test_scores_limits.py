@@ -1,4 +1,6 @@
 """Scores: what is refused, and that it is refused before anything has run (no GPU is needed)."""
+import subprocess
+import sys
 from types import SimpleNamespace
 
 import pytest
@@ -26,3 +28,20 @@ def test_a_scheduler_refuses_alternatives_when_a_request_is_submitted(n):
     with pytest.raises(ValueError, match="alternatives"):
         sch.submit(Request("r", [1, 2], 4, 0, SampleParams(logprobs=n)))
     assert not sch.queue
+
+
+_PLANS = """
+import ctypes
+from infer_b200.csrc.build import load_module
+act, i64 = load_module("act_tc"), ctypes.c_int64
+w, s, c = ctypes.c_int(), ctypes.c_int(), ctypes.c_int64()
+for M, N, K, sms in ((1 << 29, 1 << 29, 64, 148), ((1 << 30) - 1, (1 << 30) - 1, 8, 148), (100, 100, 64, 1), (100, 100, 64, 0), (1 << 29, 1 << 29, 64, 1)):
+    assert act.ib_linear_act_plan(i64(M), i64(N), i64(K), sms, ctypes.byref(w), ctypes.byref(s), ctypes.byref(c)) < 0 and act.ib_last_error()
+print("refused")
+"""
+
+
+def test_plans_that_no_width_fits_are_refused():
+    """In a process of its own: a division by a width that was never set ends one."""
+    proc = subprocess.run([sys.executable, "-c", _PLANS], capture_output=True, text=True, timeout=300)
+    assert proc.returncode == 0 and proc.stdout == "refused\n", (proc.returncode, proc.stderr[-300:])
