@@ -63,6 +63,10 @@ def main(argv=None) -> int:
         args.model = None
     elif not args.model:
         ap.error("no model: give --model DIR, --random SPEC, or set LLM_MODEL")
+    if args.logprobs is not None and not 0 <= args.logprobs <= 20:
+        ap.error(f"--logprobs takes 0 to 20, not {args.logprobs}")
+    if args.logprobs is not None and opt["cache"] == "off":
+        ap.error("--logprobs needs the cache on")
     if opt["device"] != "gpu":
         print("generate: device=cpu is not available: this engine has no CPU path", file=sys.stderr)
         return 2

@@ -45,3 +45,11 @@ def test_plans_that_no_width_fits_are_refused():
     """In a process of its own: a division by a width that was never set ends one."""
     proc = subprocess.run([sys.executable, "-c", _PLANS], capture_output=True, text=True, timeout=300)
     assert proc.returncode == 0 and proc.stdout == "refused\n", (proc.returncode, proc.stderr[-300:])
+
+
+@pytest.mark.parametrize("argv,what", [(["--logprobs", "21"], "0 to 20"), (["--logprobs", "-1"], "0 to 20"), (["cache=off", "--logprobs", "3"], "cache")])
+def test_generate_says_what_it_cannot_do(argv, what, capsys):
+    from infer_b200.cli import generate
+    with pytest.raises(SystemExit) as end:
+        generate.main(["--random", "tiny-a", *argv])
+    assert end.value.code == 2 and what in capsys.readouterr().err
