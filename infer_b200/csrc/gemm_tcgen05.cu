@@ -322,7 +322,6 @@ __device__ __forceinline__ void epilogue_store(const GemmParams& p, const float*
             float x[16];
 #pragma unroll
             for (int j = 0; j < 16; j++) x[j] = v[j] + (p.bias ? p.bias[n0 + j] : 0.0f);
-            IB_ACTIVATE_ALL(p, x);
             if (p.residual) {
                 const float4* r4 = reinterpret_cast<const float4*>(p.residual + m * p.N + n0);
 #pragma unroll
@@ -351,16 +350,13 @@ __device__ __forceinline__ void epilogue_store(const GemmParams& p, const float*
                 }
             }
         } else {
-            float x[16];
-#pragma unroll
-            for (int j = 0; j < 16; j++) x[j] = v[j] + (p.bias && n0 + j < p.N ? p.bias[n0 + j] : 0.0f);
-            IB_ACTIVATE_ALL(p, x);
 #pragma unroll
             for (int j = 0; j < 16; j++) {
                 const int64_t n = n0 + j;
                 if (n < p.N && j < ncols) {
-                    if (p.residual) x[j] += p.residual[m * p.N + n];
-                    store_elem<TOut>(out + m * p.N + n, x[j]);
+                    float x = v[j] + (p.bias ? p.bias[n] : 0.0f);
+                    if (p.residual) x += p.residual[m * p.N + n];
+                    store_elem<TOut>(out + m * p.N + n, x);
                 }
             }
         }
