@@ -32,7 +32,7 @@ __device__ __forceinline__ uint32_t map_cluster(uint32_t local_smem, uint32_t ra
     return remote;
 }
 // Says that tensor memory was read (the reads were awaited, and fenced): no other memory is handed over, so nothing is released. With a release at
-// cluster scope this took 1,100 cycles, in which the warp waits for all it has under way.
+// cluster scope this took 1,100 cycles, in which the warp waits for all it has under way. The issuer waits for each of them, the last ones behind its loop.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t remote_bar) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote_bar) : "memory");
 }

@@ -8,7 +8,8 @@
 //
 // The tensor core's additions into an accumulator truncate, and the error of a long chain has one sign: 1e-5 of the result after 8,960 elements of
 // K. Where the result is float (SUMS), an accumulator starts anew every 768 elements (below 1e-6) and the warps add what it holds to sums in
-// registers: 128 a thread, which is why a thread has half of a row's columns. The additions run under the next 768 elements' MMAs.
+// registers: 128 a thread, which is why a thread has half of a row's columns. The additions run under the next 768 elements' MMAs. A 16-bit result keeps one chain
+// (its half step is 2e-3): at 2048 x 18944 x 3584, relu squared, 0.19 % of the results are the neighbour of the correctly rounded one (sums in 32 bits: 0.03 %).
 //
 // A long K on few tiles is cut into S = 2 or 4 slices, the pairs of a cluster of 2 S CTAs. Each adds up its slice in registers; when all MMAs of
 // the cluster are done, every CTA pushes its columns to the CTAs that own them (a quarter or half each, of its own rows) through

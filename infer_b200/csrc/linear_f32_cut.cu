@@ -367,7 +367,7 @@ int launch_cut(const CUtensorMap& ma, const CUtensorMap& mb, const CutParams& p,
 // 301 x 2301 x 1000 41, 28.7, 30.7, 34.8; 257 x 5000 x 3000 207, 151, 122, 135.
 IB_EXPORT int ib_linear_f32_cut_plan(int64_t M, int64_t N, int64_t K, int sms, int* width, int64_t* scratch, int64_t* ns) {
     if (M <= 0 || N <= 0 || K <= 0) return ib::fail(IB_ERR_ARG, "linear_f32_cut: sizes must be positive");
-    // (K: a tile whose results are all computed again takes 4096 plain products a warp, while the issuer waits about a second)
+    // (K: a tile whose results are all computed again takes 4096 plain products a warp, 137 ms at 16,384 on all SMs at once, while the issuer waits about a second)
     if (M > 600000000 || N > 600000000 || K > 16384 || sms < 2) return ib::fail(IB_ERR_ARG, "linear_f32_cut: a size is too large");
     const int64_t tm = (M + 2 * BM - 1) / (2 * BM), blocks = (K + BK - 1) / BK, pitch = (K + 7) / 8 * 8;
     int64_t least = -1;

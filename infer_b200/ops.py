@@ -412,7 +412,7 @@ def head_logprobs(x: torch.Tensor, w: torch.Tensor, tokens: Optional[torch.Tenso
     """``token_logprobs`` of the logits x @ w.T (x [T, H], w [V, H], both bfloat16 or both float32; scaled and capped as there), which are
     not kept: bfloat16 rows go through a kernel that holds them in tensor memory only; up to 8 rows, rows that do not keep to 16 bytes and
     float32 go through logits of a few rows at a time. ``w`` is a loaded weight (as for ``linear``). A kernel whose bounded wait runs out
-    says so in the device's status word."""
+    says so in the device's status word. The order of a logit's sum may depend on the number of rows."""
     if not (0 <= top <= MAX_ALTERNATIVES and distribution_in_range(scale, softcap)):
         _refuse_distribution(top, scale, softcap)
     _check_product("head_logprobs", x, w)
@@ -464,7 +464,7 @@ def linear_act(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = 
     """out = residual + act(x @ w.T + bias), rounded once. x [M, K], w [N, K], both bfloat16 or both float32; bias float32 [N]; residual float32
     [M, N] (may be ``out``); ``activation``: "none", "relu", "relu_squared" (max(z, 0)^2), "gelu_tanh"
     (0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3)))), "gelu" (0.5 z (1 + erf(z / sqrt 2))), "silu" (z / (1 + e^-z)). The result is
-    float32 or bfloat16 (default: as x; with a residual float32). ``w`` is a loaded weight (as for ``linear``). A kernel whose bounded wait
+    float32 or bfloat16 (default: as x; with a residual float32; before a bfloat16 one is rounded, its sum may be off by 1e-5 after 8,960 elements of K). ``w`` is a loaded weight (as for ``linear``). A kernel whose bounded wait
     runs out says so in the device's status word. Which kernel it is, and so the order of a row's sums, may depend on the number of rows; with ``plain`` it is
     ``linear_plain``'s product, whose order does not, with the activation in a kernel behind it."""
     act = ACTIVATIONS.get(activation)
