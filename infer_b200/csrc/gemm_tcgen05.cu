@@ -350,13 +350,15 @@ __device__ __forceinline__ void epilogue_store(const GemmParams& p, const float*
                 }
             }
         } else {
+            float x[16];
+#pragma unroll
+            for (int j = 0; j < 16; j++) x[j] = v[j] + (p.bias && n0 + j < p.N ? p.bias[n0 + j] : 0.0f);
 #pragma unroll
             for (int j = 0; j < 16; j++) {
                 const int64_t n = n0 + j;
                 if (n < p.N && j < ncols) {
-                    float x = v[j] + (p.bias ? p.bias[n] : 0.0f);
-                    if (p.residual) x += p.residual[m * p.N + n];
-                    store_elem<TOut>(out + m * p.N + n, x);
+                    if (p.residual) x[j] += p.residual[m * p.N + n];
+                    store_elem<TOut>(out + m * p.N + n, x[j]);
                 }
             }
         }
